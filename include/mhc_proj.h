@@ -34,7 +34,8 @@ extern "C" {
 
 enum {
     MHC_OK = 0,
-    MHC_ERR_INVALID_VALUE = -1, /* N < 0, a null pointer with N > 0, a negative stride or an unknown dtype */
+    MHC_ERR_INVALID_VALUE = -1, /* N < 0, a null pointer with N > 0, a negative stride, an unknown dtype, or
+                                   (residual path) a width < 1, eps < 0, p outside [0, 1] or too small a workspace */
     MHC_ERR_ITERS = -2,         /* iteration count outside the supported range */
     MHC_ERR_CAPTURE = -3        /* a first call in a CUDA context that must look up a device
                                    address was made during stream capture */
@@ -312,6 +313,87 @@ MHC_API int mhc_sinkhorn_knopp_n4_hres_backward(const float* d_G, const float* d
                                                 float* d_drms, float* d_dalpha, float* d_db, int64_t N,
                                                 int num_iters, void* d_workspace,
                                                 int64_t workspace_bytes, cudaStream_t stream);
+
+/* ---- The residual path around a sublayer of an mHC layer ------------------
+ *
+ * Rows of C elements of one storage type (`dtype`), fp32 arithmetic and sums,
+ * one rounding per output.  A row's elements are contiguous; strides are in
+ * elements and non-negative; outputs are contiguous.  C >= 1 is any width and
+ * any alignment is accepted (rows whose starts are 16-byte aligned and whose
+ * width is a multiple of 16 bytes move in 16-byte pieces).  No reference
+ * counterparts. */
+
+/* y = (x - mean) * rstd * w + b per row, rstd = 1 / sqrt(var + eps) with the
+ * biased variance.  Row k of x starts at element k * x_stride.  d_w and d_b
+ * (C elements of w_dtype) may each be null: weight 1, bias 0.  d_mean and
+ * d_rstd (N floats, what the backward takes) may each be null. */
+MHC_API int mhc_layer_norm(const void* d_x, int64_t x_stride, int dtype, const void* d_w, const void* d_b,
+                           int w_dtype, void* d_y, float* d_mean, float* d_rstd, float eps, int64_t N, int64_t C,
+                           cudaStream_t stream);
+
+/* Bytes of device workspace that mhc_layer_norm_backward needs for d_dw or
+ * d_db (partial sums over rows). */
+MHC_API int mhc_layer_norm_backward_workspace(int64_t N, int64_t C, int64_t* bytes);
+
+/* Gradients of mhc_layer_norm given g = dL/dy and the forward's mean and rstd:
+ * dx (N x C, dtype), and dw and db (C elements of w_dtype), each of which may
+ * be null.  dw and db are overwritten (zeros for N = 0).  Their sums over the
+ * rows are deterministic: the same N, C and GPU model give the same bits.
+ * The call owns the workspace until it completes on `stream`; it may be null
+ * when neither dw nor db is asked for. */
+MHC_API int mhc_layer_norm_backward(const void* d_g, int64_t g_stride, const void* d_x, int64_t x_stride, int dtype,
+                                    const float* d_mean, const float* d_rstd, const void* d_w, int w_dtype,
+                                    void* d_dx, void* d_dw, void* d_db, int64_t N, int64_t C, void* d_workspace,
+                                    int64_t workspace_bytes, cudaStream_t stream);
+
+/* Dropout from a counter-based generator: y = x * s where element e is kept,
+ * 0 where not, for `count` contiguous elements.  The 16-bit draw of element e
+ * is bits 16 (e % 8) and up of Philox4x32-10 with the counter (e / 8, offset)
+ * and the key seed; it is kept when its draw is >= limit = floor(65536 p +
+ * 1/2), and s = 65536 / (65536 - limit).  d_seed, if not null, is device
+ * memory that holds the seed instead of `seed` (so a captured graph can be
+ * replayed with another one).  The gradient is the same call on dL/dy.
+ * 0 <= p <= 1.  d_y may equal d_x; other overlaps are not allowed. */
+MHC_API int mhc_dropout(const void* d_x, void* d_y, int dtype, int64_t count, double p, int64_t seed,
+                        const int64_t* d_seed, int64_t offset, cudaStream_t stream);
+
+/* Layer norm of the weighted sum of each token's four streams: mhc_layer_norm
+ * of u[k] = sum_i h[k][i] X[k][i], without u in memory.  Stream i of token k
+ * starts at element k * token_stride + i * stream_stride of X; d_h holds N x 4
+ * contiguous weights of h_dtype. */
+MHC_API int mhc_stream_norm_n4(const void* d_X, int64_t token_stride, int64_t stream_stride, int dtype,
+                               const void* d_h, int h_dtype, const void* d_w, const void* d_b, int w_dtype,
+                               void* d_y, float* d_mean, float* d_rstd, float eps, int64_t N, int64_t C,
+                               cudaStream_t stream);
+
+MHC_API int mhc_stream_norm_n4_backward_workspace(int64_t N, int64_t C, int64_t* bytes);
+
+/* Gradients of mhc_stream_norm_n4: dX (N x 4 x C, dtype), dh (N x 4, h_dtype),
+ * and dw and db as mhc_layer_norm_backward. */
+MHC_API int mhc_stream_norm_n4_backward(const void* d_g, int64_t g_stride, const void* d_X, int64_t token_stride,
+                                        int64_t stream_stride, int dtype, const void* d_h, int h_dtype,
+                                        const float* d_mean, const float* d_rstd, const void* d_w, int w_dtype,
+                                        void* d_dX, void* d_dh, void* d_dw, void* d_db, int64_t N, int64_t C,
+                                        void* d_workspace, int64_t workspace_bytes, cudaStream_t stream);
+
+/* The residual update: out[k][i] = sum_j T[k][i][j] X[k][j] + h[k][i] drop(y[k])
+ * with drop as mhc_dropout, the element's index taken in the N x C array y
+ * (p = 0: no dropout).  X as for mhc_stream_norm_n4; row k of y starts at
+ * element k * y_stride; d_T holds N x 4 x 4 and d_h N x 4 contiguous
+ * coefficients; out is N x 4 x C. */
+MHC_API int mhc_stream_mix_n4(const void* d_X, int64_t token_stride, int64_t stream_stride, const void* d_y,
+                              int64_t y_stride, int dtype, const void* d_T, int T_dtype, const void* d_h, int h_dtype,
+                              void* d_out, double p, int64_t seed, const int64_t* d_seed, int64_t offset, int64_t N,
+                              int64_t C, cudaStream_t stream);
+
+/* Gradients of mhc_stream_mix_n4 given G = dL/dout (strided as X): dX (N x 4 x
+ * C) and dy (N x C) of dtype, dT (N x 4 x 4, T_dtype) and dh (N x 4, h_dtype). */
+MHC_API int mhc_stream_mix_n4_backward(const void* d_G, int64_t g_token_stride, int64_t g_stream_stride,
+                                       const void* d_X, int64_t token_stride, int64_t stream_stride, const void* d_y,
+                                       int64_t y_stride, int dtype, const void* d_T, int T_dtype, const void* d_h,
+                                       int h_dtype, void* d_dX, void* d_dT, void* d_dy, void* d_dh, double p,
+                                       int64_t seed, const int64_t* d_seed, int64_t offset, int64_t N, int64_t C,
+                                       cudaStream_t stream);
 
 /* Human-readable text for a return code of the functions above. */
 MHC_API const char* mhc_status_string(int status);

@@ -18,6 +18,7 @@ import shlex
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -39,11 +40,17 @@ COMMON_FLAGS = [
 # reference's build does (setup.py:28), so their exp/log/divide give its
 # results exactly.  The Sinkhorn-Knopp kernels use only explicitly rounded
 # operations and a correctly rounded reciprocal; they keep the reference's
-# flush-to-zero but take the accurate expf for the fused exp(R) kernels.
+# flush-to-zero but take the accurate expf for the fused exp(R) kernels.  The
+# residual path's kernels keep IEEE arithmetic (subnormals, division, root).
 CU_SOURCES = {
     "birkhoff_n4.cu": ["--use_fast_math"],
     "sinkhorn_n4.cu": ["-ftz=true", "-prec-div=true", "-prec-sqrt=true", "-fmad=true"],
+    "layer_norm.cu": [],
+    "dropout.cu": [],
+    "stream_mix.cu": [],
 }
+
+BINDING_SOURCES = ("torch_binding.cpp", "torch_binding_residual.cpp")
 
 LIB = os.path.join(PKG, "libmhcproj.so")
 EXT = os.path.join(PKG, "_internal" + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -67,15 +74,22 @@ def _headers() -> list[str]:
     return hs + [os.path.join(INCLUDE, "mhc_proj.h")]
 
 
+def _compile(jobs: list[list[str]], verbose: bool) -> None:
+    """Runs independent compiler commands, a few at a time."""
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(lambda cmd: _run(cmd, verbose), jobs))
+
+
 def build_cuda_lib(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    objs = []
+    objs, jobs = [], []
     for src, math_flags in CU_SOURCES.items():
         s = os.path.join(CSRC, src)
         o = os.path.join(BUILD, src.replace(".cu", ".o"))
         if force or _stale(o, [s, *_headers(), __file__]):
-            _run([NVCC, *COMMON_FLAGS, *math_flags, "-I", INCLUDE, "-I", CSRC, "-c", s, "-o", o], verbose)
+            jobs.append([NVCC, *COMMON_FLAGS, *math_flags, "-I", INCLUDE, "-I", CSRC, "-c", s, "-o", o])
         objs.append(o)
+    _compile(jobs, verbose)
     if force or _stale(LIB, objs):
         _run([NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", *objs, "-o", LIB,
               "-lcudart", "-Xlinker", "-soname=libmhcproj.so"], verbose)
@@ -83,14 +97,15 @@ def build_cuda_lib(force: bool = False, verbose: bool = True) -> str:
 
 
 def build_torch_ext(force: bool = False, verbose: bool = True) -> str:
-    src = os.path.join(CSRC, "torch_binding.cpp")
-    if not (force or _stale(EXT, [src, LIB, os.path.join(INCLUDE, "mhc_proj.h"), __file__])):
+    srcs = [os.path.join(CSRC, f) for f in BINDING_SOURCES]
+    heads = [os.path.join(CSRC, "torch_binding.h"), os.path.join(INCLUDE, "mhc_proj.h"), __file__]
+    if not (force or _stale(EXT, [*srcs, *heads, LIB])):
         return EXT
     import torch
     from torch.utils import cpp_extension as ce
 
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
              f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
              "-DTORCH_EXTENSION_NAME=_internal", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     incs = []
@@ -102,7 +117,15 @@ def build_torch_ext(force: bool = False, verbose: bool = True) -> str:
             "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
             "-L", os.path.join(CUDA_HOME, "lib64"), "-lcudart",
             "-L", PKG, "-l:libmhcproj.so", "-Wl,-rpath,$ORIGIN"]
-    _run([CXX, *flags, *incs, src, "-o", EXT, *libs], verbose)
+    os.makedirs(BUILD, exist_ok=True)
+    objs, jobs = [], []
+    for s in srcs:
+        o = os.path.join(BUILD, os.path.basename(s).replace(".cpp", ".o"))
+        if force or _stale(o, [s, *heads]):
+            jobs.append([CXX, *flags, *incs, "-c", s, "-o", o])
+        objs.append(o)
+    _compile(jobs, verbose)
+    _run([CXX, "-shared", *objs, "-o", EXT, *libs], verbose)
     return EXT
 
 

@@ -22,17 +22,10 @@
 // batch stride, instead of copying them to contiguous fp32 and back; the
 // results are the same bits.  So do the Sinkhorn-Knopp functions (other
 // layouts of those types are made contiguous in their own type first).
-#include <stdexcept>
-#include <string>
-
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <pybind11/pybind11.h>
-#include <torch/extension.h>
-
-#include "mhc_proj.h"
+#include "torch_binding.h"
 
 namespace py = pybind11;
+using namespace mhcp_torch;
 
 namespace {
 
@@ -42,34 +35,6 @@ void check_batch(const torch::Tensor& x, const char* name, int64_t batch = -1)
     if (x.dim() != 3) throw std::runtime_error(msg);
     if (x.size(1) != 4 || x.size(2) != 4) throw std::runtime_error(msg);
     if (batch >= 0 && x.size(0) != batch) throw std::runtime_error(msg);
-}
-
-// fp32 on the tensor's own CUDA device, or on the current device for
-// non-CUDA tensors (solvers_torch.cpp:52-61).
-torch::TensorOptions target_options(const torch::Tensor& x)
-{
-    auto opts = torch::TensorOptions().dtype(torch::kFloat32).device(torch::kCUDA);
-    if (x.device().is_cuda()) opts = opts.device(torch::kCUDA, x.device().index());
-    return opts;
-}
-
-void check_status(int status, const char* what)
-{
-    if (status != MHC_OK)
-        throw std::runtime_error(std::string(what) + " failed: " + mhc_status_string(status));
-}
-
-cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-
-// Storage type code of the *_ex entry points, or -1.
-int dtype_code(const torch::Tensor& x)
-{
-    switch (x.scalar_type()) {
-        case torch::kFloat32: return MHC_DTYPE_F32;
-        case torch::kBFloat16: return MHC_DTYPE_BF16;
-        case torch::kFloat16: return MHC_DTYPE_F16;
-        default: return -1;
-    }
 }
 
 // A CUDA batch the kernels read in place: a type they take and contiguous
@@ -544,4 +509,5 @@ PYBIND11_MODULE(_internal, m)
     m_torch.def("sinkhorn_knopp_n4_hres_backward", &sinkhorn_knopp_n4_hres_backward, py::arg("G"), py::arg("h_res"),
                 py::arg("rms"), py::arg("alpha_res"), py::arg("b_res"), py::arg("max_iter") = 20,
                 "Gradients of sinkhorn_knopp_n4_hres with respect to h_res, rms, alpha_res and b_res");
+    bind_residual_path(m_torch);
 }

@@ -5,7 +5,10 @@ Drop-in for the reference package of the same name (mhc_proj/__init__.py of
 Aoblex/mHC-proj): ``mhc_proj.MHCProjectionN4``, ``mhc_proj.MHCSinkhornN4`` and
 the low-level ``mhc_proj.torch.*`` functions.  ``mhc_proj.MHCProjectionN4HRes``
 and ``mhc_proj.MHCSinkhornN4HRes`` add the projection and the Sinkhorn-Knopp
-pair fused with the mHC layer's H_res producer.  The
+pair fused with the mHC layer's H_res producer.  The residual path around a
+sublayer is there as ``MHCStreamNormN4`` (the four streams read and normalised),
+``MHCStreamMixN4`` (mixed by the projected matrices, with the sublayer's output
+and its dropout added), ``MHCLayerNorm`` and ``MHCDropout``.  The
 native extension is required; there is no CPU fallback.
 """
 # torch first so that libc10 and the CUDA runtime resolve for the extension.
@@ -20,6 +23,8 @@ except ImportError as e:  # pragma: no cover - exercised only on a broken instal
         "(run `python mhc-proj_b200/build.py`): " + str(e)) from e
 
 from .module import MHCProjectionN4, MHCProjectionN4HRes, MHCSinkhornN4, MHCSinkhornN4HRes  # noqa: E402
+from .residual import MHCDropout, MHCLayerNorm, MHCStreamMixN4, MHCStreamNormN4  # noqa: E402
 
 __version__ = "0.1.0"
-__all__ = ["MHCProjectionN4", "MHCProjectionN4HRes", "MHCSinkhornN4", "MHCSinkhornN4HRes", "torch"]
+__all__ = ["MHCProjectionN4", "MHCProjectionN4HRes", "MHCSinkhornN4", "MHCSinkhornN4HRes", "MHCLayerNorm",
+           "MHCDropout", "MHCStreamNormN4", "MHCStreamMixN4", "torch"]

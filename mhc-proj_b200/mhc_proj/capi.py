@@ -36,6 +36,15 @@ EXPORTED = (
     "mhc_sinkhorn_knopp_n4_hres",
     "mhc_sinkhorn_knopp_n4_hres_backward_workspace",
     "mhc_sinkhorn_knopp_n4_hres_backward",
+    "mhc_layer_norm",
+    "mhc_layer_norm_backward_workspace",
+    "mhc_layer_norm_backward",
+    "mhc_dropout",
+    "mhc_stream_norm_n4",
+    "mhc_stream_norm_n4_backward_workspace",
+    "mhc_stream_norm_n4_backward",
+    "mhc_stream_mix_n4",
+    "mhc_stream_mix_n4_backward",
     "mhc_status_string",
     "mhc_abi_version",
 )
@@ -92,6 +101,19 @@ def lib() -> ctypes.CDLL:
         L.mhc_sinkhorn_knopp_n4_hres_backward_workspace.argtypes = [i64, ctypes.POINTER(i64)]
         L.mhc_sinkhorn_knopp_n4_hres_backward.argtypes = [vp, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i64, i32,
                                                           vp, i64, vp]
+        f64, out64 = ctypes.c_double, ctypes.POINTER(i64)
+        L.mhc_layer_norm.argtypes = [vp, i64, i32, vp, vp, i32, vp, vp, vp, f32, i64, i64, vp]
+        L.mhc_layer_norm_backward_workspace.argtypes = [i64, i64, out64]
+        L.mhc_layer_norm_backward.argtypes = [vp, i64, vp, i64, i32, vp, vp, vp, i32, vp, vp, vp, i64, i64, vp, i64, vp]
+        L.mhc_dropout.argtypes = [vp, vp, i32, i64, f64, i64, vp, i64, vp]
+        L.mhc_stream_norm_n4.argtypes = [vp, i64, i64, i32, vp, i32, vp, vp, i32, vp, vp, vp, f32, i64, i64, vp]
+        L.mhc_stream_norm_n4_backward_workspace.argtypes = [i64, i64, out64]
+        L.mhc_stream_norm_n4_backward.argtypes = [vp, i64, vp, i64, i64, i32, vp, i32, vp, vp, vp, i32, vp, vp, vp, vp,
+                                                  i64, i64, vp, i64, vp]
+        L.mhc_stream_mix_n4.argtypes = [vp, i64, i64, vp, i64, i32, vp, i32, vp, i32, vp, f64, i64, vp, i64, i64, i64,
+                                        vp]
+        L.mhc_stream_mix_n4_backward.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, i32, vp, i32, vp, i32, vp, vp, vp,
+                                                 vp, f64, i64, vp, i64, i64, i64, vp]
         for f in _LAUNCHERS:
             getattr(L, f).restype = ctypes.c_int
         L.mhc_status_string.argtypes = [ctypes.c_int]
@@ -236,6 +258,74 @@ def sinkhorn_knopp_n4_hres_backward(G: int, h: int, h_stride: int, rms: int, alp
     _check(lib().mhc_sinkhorn_knopp_n4_hres_backward(G, h, h_stride, rms, alpha, b, dh, dh_stride, drms, dalpha,
                                                       db, N, num_iters, workspace, workspace_bytes, stream),
            "mhc_sinkhorn_knopp_n4_hres_backward")
+
+
+# --- the residual path (pointers may be 0 where the header allows null) -------
+
+def layer_norm(x: int, x_stride: int, dtype: int, w: int, b: int, w_dtype: int, y: int, mean: int, rstd: int,
+               eps: float, N: int, C: int, stream: int = 0) -> None:
+    _check(lib().mhc_layer_norm(x, x_stride, dtype, w, b, w_dtype, y, mean, rstd, eps, N, C, stream), "mhc_layer_norm")
+
+
+def layer_norm_backward_workspace(N: int, C: int) -> int:
+    """Bytes of workspace mhc_layer_norm_backward needs for N rows of C elements."""
+    out = ctypes.c_int64(0)
+    _check(lib().mhc_layer_norm_backward_workspace(N, C, ctypes.byref(out)), "mhc_layer_norm_backward_workspace")
+    return out.value
+
+
+def layer_norm_backward(g: int, g_stride: int, x: int, x_stride: int, dtype: int, mean: int, rstd: int, w: int,
+                        w_dtype: int, dx: int, dw: int, db: int, N: int, C: int, workspace: int, workspace_bytes: int,
+                        stream: int = 0) -> None:
+    _check(lib().mhc_layer_norm_backward(g, g_stride, x, x_stride, dtype, mean, rstd, w, w_dtype, dx, dw, db, N, C,
+                                         workspace, workspace_bytes, stream),
+           "mhc_layer_norm_backward")
+
+
+def dropout(x: int, y: int, dtype: int, count: int, p: float, seed: int, seed_ptr: int = 0, offset: int = 0,
+            stream: int = 0) -> None:
+    """seed_ptr: device memory that holds the seed (0: `seed` is it)."""
+    _check(lib().mhc_dropout(x, y, dtype, count, p, seed, seed_ptr, offset, stream), "mhc_dropout")
+
+
+def stream_norm_n4(X: int, token_stride: int, stream_stride: int, dtype: int, h: int, h_dtype: int, w: int, b: int,
+                   w_dtype: int, y: int, mean: int, rstd: int, eps: float, N: int, C: int, stream: int = 0) -> None:
+    _check(lib().mhc_stream_norm_n4(X, token_stride, stream_stride, dtype, h, h_dtype, w, b, w_dtype, y, mean, rstd,
+                                    eps, N, C, stream),
+           "mhc_stream_norm_n4")
+
+
+def stream_norm_n4_backward_workspace(N: int, C: int) -> int:
+    out = ctypes.c_int64(0)
+    _check(lib().mhc_stream_norm_n4_backward_workspace(N, C, ctypes.byref(out)),
+           "mhc_stream_norm_n4_backward_workspace")
+    return out.value
+
+
+def stream_norm_n4_backward(g: int, g_stride: int, X: int, token_stride: int, stream_stride: int, dtype: int, h: int,
+                            h_dtype: int, mean: int, rstd: int, w: int, w_dtype: int, dX: int, dh: int, dw: int,
+                            db: int, N: int, C: int, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    _check(lib().mhc_stream_norm_n4_backward(g, g_stride, X, token_stride, stream_stride, dtype, h, h_dtype, mean, rstd,
+                                             w, w_dtype, dX, dh, dw, db, N, C, workspace, workspace_bytes, stream),
+           "mhc_stream_norm_n4_backward")
+
+
+def stream_mix_n4(X: int, token_stride: int, stream_stride: int, y: int, y_stride: int, dtype: int, T: int,
+                  T_dtype: int, h: int, h_dtype: int, out: int, p: float, seed: int, seed_ptr: int, offset: int, N: int,
+                  C: int, stream: int = 0) -> None:
+    _check(lib().mhc_stream_mix_n4(X, token_stride, stream_stride, y, y_stride, dtype, T, T_dtype, h, h_dtype, out, p,
+                                   seed, seed_ptr, offset, N, C, stream),
+           "mhc_stream_mix_n4")
+
+
+def stream_mix_n4_backward(G: int, g_token_stride: int, g_stream_stride: int, X: int, token_stride: int,
+                           stream_stride: int, y: int, y_stride: int, dtype: int, T: int, T_dtype: int, h: int,
+                           h_dtype: int, dX: int, dT: int, dy: int, dh: int, p: float, seed: int, seed_ptr: int,
+                           offset: int, N: int, C: int, stream: int = 0) -> None:
+    _check(lib().mhc_stream_mix_n4_backward(G, g_token_stride, g_stream_stride, X, token_stride, stream_stride, y,
+                                            y_stride, dtype, T, T_dtype, h, h_dtype, dX, dT, dy, dh, p, seed, seed_ptr,
+                                            offset, N, C, stream),
+           "mhc_stream_mix_n4_backward")
 
 
 # --- tensor conveniences ---------------------------------------------------
