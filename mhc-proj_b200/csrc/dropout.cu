@@ -10,18 +10,55 @@
 namespace mhcp {
 
 constexpr int kDropBlock = 256;
+constexpr int kDropGroups = 4;  // groups a thread takes
 
-// One thread takes a group of eight elements, one counter's draws.
+// A group of eight elements, one counter's draws, from and to 16-byte aligned memory.
+template <class Elem>
+struct Group {
+    static constexpr int kPieces = 8 * sizeof(Elem) / 16;
+    uint4 q[kPieces];
+
+    __device__ __forceinline__ void load(const Elem* p)
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void store(Elem* p) const
+    {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p)[i] = q[i];
+    }
+    __device__ __forceinline__ void drop(uint32_t keep, float scale)
+    {
+        Elem* e = reinterpret_cast<Elem*>(q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_f32<Elem>((keep >> i & 1u) ? to_f32(e[i]) * scale : 0.0f);
+    }
+};
+
 template <class Elem, bool kVec>
 __global__ void __launch_bounds__(kDropBlock)
 dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
 {
     const uint2 key = dropout_key(d);
-    const int64_t groups = ceil_div(count, 8);
-    for (int64_t q = blockIdx.x * static_cast<int64_t>(kDropBlock) + threadIdx.x; q < groups;
-         q += gridDim.x * static_cast<int64_t>(kDropBlock)) {
+    const int64_t q0 = blockIdx.x * static_cast<int64_t>(kDropBlock * kDropGroups) + threadIdx.x;
+    const int64_t whole = count / 8;
+    if (kVec && q0 + (kDropGroups - 1) * kDropBlock < whole) {
+        Group<Elem> g[kDropGroups];
+#pragma unroll
+        for (int k = 0; k < kDropGroups; ++k) g[k].load(x + 8 * (q0 + k * kDropBlock));
+#pragma unroll
+        for (int k = 0; k < kDropGroups; ++k) {
+            const int64_t q = q0 + k * kDropBlock;
+            g[k].drop(d.limit ? keep_bits(q, d.offset, key, d.limit) : 0xffu, d.scale);
+            g[k].store(y + 8 * q);
+        }
+        return;
+    }
+    for (int k = 0; k < kDropGroups; ++k) {
+        const int64_t q = q0 + k * kDropBlock, e = 8 * q;
+        if (e >= count) return;
         const uint32_t keep = d.limit ? keep_bits(q, d.offset, key, d.limit) : 0xffu;
-        const int64_t e = 8 * q;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (e + i < count) y[e + i] = from_f32<Elem>((keep >> i & 1u) ? to_f32(x[e + i]) * d.scale : 0.0f);
@@ -31,9 +68,14 @@ dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
 template <class Elem>
 static int dropout_launch(const void* x, void* y, int64_t count, const Dropout& d, cudaStream_t stream)
 {
-    const int64_t blocks = std::min(ceil_div(ceil_div(count, 8), kDropBlock), int64_t{1} << 30);
-    dropout_kernel<Elem, false><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(
-        static_cast<const Elem*>(x), static_cast<Elem*>(y), count, d);
+    const int64_t blocks = ceil_div(count, 8 * kDropBlock * kDropGroups);
+    if (blocks > 0x7fffffff) return MHC_ERR_INVALID_VALUE;
+    const Elem* xe = static_cast<const Elem*>(x);
+    Elem* ye = static_cast<Elem*>(y);
+    if (aligned16(x) && aligned16(y))
+        dropout_kernel<Elem, true><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(xe, ye, count, d);
+    else
+        dropout_kernel<Elem, false><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(xe, ye, count, d);
     return static_cast<int>(cudaGetLastError());
 }
 

@@ -13,53 +13,22 @@
 // squared distances from the mean (never a difference of squares, which
 // cancels for rows far from zero).
 #include <algorithm>
+#include <type_traits>
 
+#include "norm_ring.cuh"
+#include "norm_source.cuh"
 #include "row_ops.cuh"
 
 namespace mhcp {
 
+#ifndef MHC_RING_N
+#define MHC_RING_N 1024
+#endif
+#ifndef MHC_NORM_E16
+#define MHC_NORM_E16 1
+#endif
 constexpr int kNormBlock = 256;
-
-// Where a row's u comes from: one row, or four weighted ones.
-template <class Elem, int kStreams>
-struct NormSource {
-    const Elem* x;
-    int64_t stride, stream_stride;
-    const void* h;
-    int h_dtype;
-};
-
-template <class Elem, int kStreams>
-struct NormRow {
-    const Elem* x;
-    int64_t stream_stride;
-    float h[kStreams];
-
-    __device__ __forceinline__ NormRow(const NormSource<Elem, kStreams>& s, int64_t r)
-        : x(s.x + r * s.stride), stream_stride(s.stream_stride)
-    {
-        if constexpr (kStreams == 1) {
-            h[0] = 1.0f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < kStreams; ++i) h[i] = load_any(s.h, r * kStreams + i, s.h_dtype);
-        }
-    }
-
-    __device__ __forceinline__ float at(int64_t c) const
-    {
-        if constexpr (kStreams == 1) return to_f32(x[c]);
-        float u = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kStreams; ++i) u = fmaf(h[i], to_f32(x[i * stream_stride + c]), u);
-        return u;
-    }
-};
-
-struct NormAffine {
-    const void *w, *b;
-    int dtype;
-};
+constexpr int kHeldThreads = 512;
 
 // One block per row, which it reads three times (the second and third come
 // from L1 or L2).
@@ -92,6 +61,125 @@ norm_fwd_rows(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__
             if (mean_out) mean_out[r] = mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
+    }
+}
+
+// The columns of a thread in a group of blockDim.x threads that hold a whole
+// row: piece p of kPieces.
+template <class Elem, bool kVec>
+struct HeldCols;
+template <class Elem>
+struct HeldCols<Elem, true> {
+    using Cols = VecCols<Elem>;
+    static __device__ __forceinline__ Cols cols(int p, int C)
+    {
+        const int c = (p * blockDim.x + threadIdx.x) * Cols::K;
+        return Cols(c, c < C);
+    }
+};
+template <class Elem>
+struct HeldCols<Elem, false> {
+    using Cols = LooseCols<Elem, 8>;
+    static __device__ __forceinline__ Cols cols(int p, int C)
+    {
+        return Cols(p * 8 * blockDim.x + threadIdx.x, blockDim.x, C);
+    }
+};
+
+// w or b at a thread's columns; `none` where there is no such array.
+template <class Elem, bool kVec, class Cols>
+__device__ __forceinline__ void load_param(const void* p, int dtype, const Cols& cols, float none, float (&v)[Cols::K])
+{
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < Cols::K; ++j) v[j] = none;
+        return;
+    }
+    if constexpr (kVec) {
+        // of x's own type, or fp32 (the launcher's rule): 16-byte pieces
+        if (sizeof(Elem) == 4 || dtype != MHC_DTYPE_F32) {
+            cols.load(static_cast<const Elem*>(p), v);
+        } else {
+            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + cols.c0);
+#pragma unroll
+            for (int i = 0; i < Cols::K / 4; ++i) {
+                const float4 f = cols.c0 >= 0 ? __ldg(q + i) : make_float4(0, 0, 0, 0);
+                v[4 * i] = f.x;
+                v[4 * i + 1] = f.y;
+                v[4 * i + 2] = f.z;
+                v[4 * i + 3] = f.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < Cols::K; ++j) v[j] = cols.has(j) ? load_any(p, cols.col(j), dtype) : none;
+    }
+}
+
+// A row held in the registers of blockDim.x threads, read once; blockDim.y
+// rows a block (more than one only where a row is one warp's).
+template <class Elem, int kStreams, bool kVec, int kElems>
+__global__ void __launch_bounds__(kHeldThreads)
+norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
+              float* __restrict__ rstd_out, float eps, int64_t N, int C)
+{
+    using Held = HeldCols<Elem, kVec>;
+    using Cols = typename Held::Cols;
+    constexpr int K = Cols::K, P = kElems / K;
+    __shared__ float buf[2][32];
+    const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
+    if (r >= N) return;
+    const NormRow<Elem, kStreams> row(src, r);
+    float u[P][K];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const Cols cols = Held::cols(p, C);
+        cols.load(row.x, u[p]);
+        if constexpr (kStreams > 1) {
+            float v[kStreams - 1][K];
+#pragma unroll
+            for (int i = 1; i < kStreams; ++i) cols.load(row.x + i * row.stream_stride, v[i - 1]);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                u[p][j] *= row.h[0];
+#pragma unroll
+                for (int i = 1; i < kStreams; ++i) u[p][j] = fmaf(row.h[i], v[i - 1][j], u[p][j]);
+            }
+        }
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) s[0] += u[p][j];
+    }
+    block_sum(s, buf[0]);
+    const float inv = 1.0f / static_cast<float>(C), mean = s[0] * inv;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const Cols cols = Held::cols(p, C);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            u[p][j] = cols.has(j) ? u[p][j] - mean : 0.0f;
+            s[0] = fmaf(u[p][j], u[p][j], s[0]);
+        }
+    }
+    block_sum(s, buf[1]);
+    const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const Cols cols = Held::cols(p, C);
+        float w[K], b[K];
+        load_param<Elem, kVec>(aff.w, aff.dtype, cols, 1.0f, w);
+        load_param<Elem, kVec>(aff.b, aff.dtype, cols, 0.0f, b);
+#pragma unroll
+        for (int j = 0; j < K; ++j) w[j] = fmaf(u[p][j] * rstd, w[j], b[j]);
+        cols.store(y + r * C, w);
+    }
+    if (threadIdx.x == 0) {
+        if (mean_out) mean_out[r] = mean;
+        if (rstd_out) rstd_out[r] = rstd;
     }
 }
 
@@ -205,10 +293,92 @@ norm_param_fold(const float* __restrict__ partials, int64_t rows, void* __restri
 constexpr int64_t kMaxRowGrid = int64_t{1} << 20;
 constexpr int64_t kParamChunks = 64;
 
+// Rows of partial sums at most: the row kernels' chunks, or the ring kernel's blocks.
+constexpr int64_t kMaxPartials = 1024;
+
 static int64_t norm_workspace(int64_t N, int64_t C)
 {
-    return std::max<int64_t>(1, std::min(ceil_div(N, kParamRows), kParamChunks)) * 2 * C *
-           static_cast<int64_t>(sizeof(float));
+    return std::max<int64_t>(1, std::min(N, kMaxPartials)) * 2 * C * static_cast<int64_t>(sizeof(float));
+}
+
+// Whether rows move in 16-byte pieces: whole pieces, aligned, and the
+// parameters of a type that load_param reads in pieces.
+template <class Elem, int kStreams>
+static bool norm_in_pieces(const NormSource<Elem, kStreams>& src, const NormAffine& aff, int64_t C)
+{
+    constexpr int e = sizeof(Elem);
+    const int own = e == 4 ? MHC_DTYPE_F32 : std::is_same<Elem, __half>::value ? MHC_DTYPE_F16 : MHC_DTYPE_BF16;
+    return ((C * e) & 15) == 0 && aligned16(src.x, src.stride, e) && ((src.stream_stride * e) & 15) == 0 &&
+           aligned16(aff.w) && aligned16(aff.b) &&
+           ((!aff.w && !aff.b) || aff.dtype == own || aff.dtype == MHC_DTYPE_F32);
+}
+
+// The widest row that a block holds.
+constexpr int64_t kHeldMax = 32 * kHeldThreads;
+
+template <class Elem, int kStreams, bool kVec, int kElems>
+static void norm_forward_held(const NormSource<Elem, kStreams>& src, const NormAffine& aff, Elem* y, float* mean,
+                              float* rstd, float eps, int64_t N, int64_t C, cudaStream_t stream)
+{
+    const int t = 32 * static_cast<int>(ceil_div(C, 32 * kElems));
+    const int per_block = t == 32 ? 4 : 1;
+    norm_fwd_held<Elem, kStreams, kVec, kElems>
+        <<<static_cast<unsigned>(ceil_div(N, per_block)), dim3(t, per_block), 0, stream>>>(
+            src, aff, y, mean, rstd, eps, N, static_cast<int>(C));
+}
+
+// The ring kernels' shape for rows of C elements.
+struct RingPlan {
+    int threads, groups, stages, blocks_per_sm, smem;
+};
+
+constexpr int kRingElems = 16;                // of a row, per thread
+constexpr int64_t kRingMax = 1024 * kRingElems;
+constexpr int kRingSmem = 200 * 1024;         // of an SM's 227 KB, for the ring
+
+static RingPlan ring_plan(int64_t C, int elem, bool vec, int rows, int threads_per_sm)
+{
+    RingPlan p;
+    p.threads = 32 * static_cast<int>(ceil_div(C, 32 * kRingElems));
+    p.groups = p.threads == 32 ? 4 : 1;
+    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, vec, p.threads, kRingElems) * p.groups;
+    p.blocks_per_sm = std::max(1, std::min(threads_per_sm / (p.threads * p.groups), kRingSmem / (2 * stage)));
+    p.stages = std::min(kRingStages, std::max(1, kRingSmem / p.blocks_per_sm / stage));
+    p.smem = std::max(p.stages * stage, p.groups > 1 ? static_cast<int>(8 * C) : 0);
+    if (stage > 225 * 1024) p.stages = 0;  // one row does not fit
+    return p;
+}
+
+static int sm_count()
+{
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    return sms;
+}
+
+// A launch may need more dynamic shared memory than a kernel has by default;
+// the attribute belongs to the context, so it is set for each such launch.
+template <class Kernel>
+static cudaError_t allow_smem(Kernel kernel, int bytes)
+{
+    return bytes <= 44 * 1024 ? cudaSuccess  // 48 KB less what is static
+                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <class Elem, int kStreams, bool kVec>
+static cudaError_t norm_forward_ring(const RingPlan& p, const NormSource<Elem, kStreams>& src, const NormAffine& aff,
+                                     Elem* y, float* mean, float* rstd, float eps, int64_t N, int64_t C,
+                                     cudaStream_t stream)
+{
+    const auto kernel = norm_fwd_ring<Elem, kStreams, kVec, kRingElems>;
+    const cudaError_t e = allow_smem(kernel, p.smem);
+    if (e != cudaSuccess) return e;
+    const int64_t grid = std::min<int64_t>(ceil_div(N, p.groups), static_cast<int64_t>(p.blocks_per_sm) * sm_count());
+    kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
+        src, span_of(src.x, N, src.stride, kStreams, src.stream_stride, C), aff, y, mean, rstd, eps, N,
+        static_cast<int>(C), p.stages);
+    return cudaSuccess;
 }
 
 template <class Elem, int kStreams>
@@ -217,8 +387,25 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, co
                         cudaStream_t stream)
 {
     const NormSource<Elem, kStreams> src{static_cast<const Elem*>(x), stride, stream_stride, h, h_dtype};
-    norm_fwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
-        src, aff, static_cast<Elem*>(y), mean, rstd, eps, N, C);
+    Elem* yp = static_cast<Elem*>(y);
+    const bool pieces = norm_in_pieces(src, aff, C) && aligned16(y);
+    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams, 768);
+    if (C <= kRingMax && plan.stages > 0 && N >= MHC_RING_N) {
+        const cudaError_t e = pieces ? norm_forward_ring<Elem, kStreams, true>(plan, src, aff, yp, mean, rstd, eps, N, C, stream)
+                                     : norm_forward_ring<Elem, kStreams, false>(plan, src, aff, yp, mean, rstd, eps, N, C, stream);
+        if (e != cudaSuccess) return static_cast<int>(e);
+    } else if (C > kHeldMax)
+        norm_fwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
+            src, aff, yp, mean, rstd, eps, N, C);
+    else if (C > 16 * kHeldThreads)
+        pieces ? norm_forward_held<Elem, kStreams, true, 32>(src, aff, yp, mean, rstd, eps, N, C, stream)
+               : norm_forward_held<Elem, kStreams, false, 32>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    else if (MHC_NORM_E16 || C > 8 * kHeldThreads)
+        pieces ? norm_forward_held<Elem, kStreams, true, 16>(src, aff, yp, mean, rstd, eps, N, C, stream)
+               : norm_forward_held<Elem, kStreams, false, 16>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    else
+        pieces ? norm_forward_held<Elem, kStreams, true, 8>(src, aff, yp, mean, rstd, eps, N, C, stream)
+               : norm_forward_held<Elem, kStreams, false, 8>(src, aff, yp, mean, rstd, eps, N, C, stream);
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -227,7 +414,7 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, in
                         const void* w, const void* b, int w_dtype, void* y, float* mean, float* rstd, float eps,
                         int64_t N, int64_t C, cudaStream_t stream)
 {
-    if (N < 0 || C < 1 || stride < 0 || stream_stride < 0 || !known_dtype(dtype) || !known_dtype(h_dtype) ||
+    if (N < 0 || N >= (int64_t{1} << 31) || C < 1 || C > kMaxWidth || stride < 0 || stream_stride < 0 || !known_dtype(dtype) || !known_dtype(h_dtype) ||
         !known_dtype(w_dtype) || !(eps >= 0.0f) || (N > 0 && (!x || !y || (kStreams > 1 && !h))))
         return MHC_ERR_INVALID_VALUE;
     if (N == 0) return MHC_OK;
@@ -245,6 +432,22 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, in
     }
 }
 
+template <class Elem, int kStreams, bool kVec, int kMaxThreads>
+static cudaError_t norm_backward_ring(const RingPlan& p, int64_t grid, const Elem* g, int64_t g_stride,
+                                      const NormSource<Elem, kStreams>& src, const float* mean, const float* rstd,
+                                      const NormAffine& aff, Elem* dx, void* dh, float* partials, int64_t N, int64_t C,
+                                      cudaStream_t stream)
+{
+    const auto kernel = norm_bwd_ring<Elem, kStreams, kVec, kRingElems, kMaxThreads>;
+    const cudaError_t e = allow_smem(kernel, p.smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
+        g, g_stride, span_of(g, N, g_stride, 1, 0, C), src,
+        span_of(src.x, N, src.stride, kStreams, src.stream_stride, C), mean, rstd, aff, dx, dh, partials, N,
+        static_cast<int>(C), p.stages);
+    return cudaSuccess;
+}
+
 template <class Elem, int kStreams>
 static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t stride, int64_t stream_stride,
                          const void* h, int h_dtype, const float* mean, const float* rstd, const NormAffine& aff,
@@ -253,11 +456,28 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
 {
     const NormSource<Elem, kStreams> src{static_cast<const Elem*>(x), stride, stream_stride, h, h_dtype};
     const Elem* gp = static_cast<const Elem*>(g);
+    const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
+    const bool pieces = norm_in_pieces(src, aff, C) && aligned16(g, g_stride, sizeof(Elem)) && aligned16(dx);
+    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams + 1, 512);
+    if (N > 0 && C <= kRingMax && plan.stages > 0) {
+        const int64_t grid = std::min(
+            {ceil_div(N, plan.groups), static_cast<int64_t>(plan.blocks_per_sm) * sm_count(), kMaxPartials});
+        float* part = dw || db ? partials : nullptr;
+        Elem* dxp = static_cast<Elem*>(dx);
+        const bool wide = plan.threads > 512;
+        const cudaError_t e =
+            pieces ? (wide ? norm_backward_ring<Elem, kStreams, true, 1024>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream)
+                           : norm_backward_ring<Elem, kStreams, true, 512>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream))
+                   : (wide ? norm_backward_ring<Elem, kStreams, false, 1024>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream)
+                           : norm_backward_ring<Elem, kStreams, false, 512>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream));
+        if (e != cudaSuccess) return static_cast<int>(e);
+        if (part) norm_param_fold<<<dim3(cols, 2), 32 * kParamRows, 0, stream>>>(partials, grid, dw, db, aff.dtype, C);
+        return static_cast<int>(cudaGetLastError());
+    }
     if (N > 0)
         norm_bwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
             gp, g_stride, src, mean, rstd, aff, static_cast<Elem*>(dx), dh, N, C);
     if (dw || db) {
-        const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
         int64_t chunks = 0;
         if (N > 0) {
             chunks = std::min(ceil_div(N, kParamRows), kParamChunks);
@@ -277,7 +497,7 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
                          int w_dtype, void* dx, void* dh, void* dw, void* db, int64_t N, int64_t C, void* workspace,
                          int64_t workspace_bytes, cudaStream_t stream)
 {
-    if (N < 0 || C < 1 || g_stride < 0 || stride < 0 || stream_stride < 0 || !known_dtype(dtype) ||
+    if (N < 0 || N >= (int64_t{1} << 31) || C < 1 || C > kMaxWidth || g_stride < 0 || stride < 0 || stream_stride < 0 || !known_dtype(dtype) ||
         !known_dtype(h_dtype) || !known_dtype(w_dtype) ||
         (N > 0 && (!g || !x || !mean || !rstd || !dx || (kStreams > 1 && (!h || !dh)))))
         return MHC_ERR_INVALID_VALUE;
@@ -312,7 +532,7 @@ extern "C" int mhc_layer_norm(const void* d_x, int64_t x_stride, int dtype, cons
 
 extern "C" int mhc_layer_norm_backward_workspace(int64_t N, int64_t C, int64_t* bytes)
 {
-    if (N < 0 || C < 1 || !bytes) return MHC_ERR_INVALID_VALUE;
+    if (N < 0 || N >= (int64_t{1} << 31) || C < 1 || C > kMaxWidth || !bytes) return MHC_ERR_INVALID_VALUE;
     *bytes = norm_workspace(N, C);
     return MHC_OK;
 }
@@ -337,7 +557,7 @@ extern "C" int mhc_stream_norm_n4(const void* d_X, int64_t token_stride, int64_t
 
 extern "C" int mhc_stream_norm_n4_backward_workspace(int64_t N, int64_t C, int64_t* bytes)
 {
-    if (N < 0 || C < 1 || !bytes) return MHC_ERR_INVALID_VALUE;
+    if (N < 0 || N >= (int64_t{1} << 31) || C < 1 || C > kMaxWidth || !bytes) return MHC_ERR_INVALID_VALUE;
     *bytes = norm_workspace(N, C);
     return MHC_OK;
 }

@@ -43,97 +43,273 @@ __device__ __forceinline__ MixCoef mix_coef(const MixIn<Elem>& in, int64_t r)
     return k;
 }
 
-// drop's factor of element e.
-__device__ __forceinline__ float drop_factor(int64_t e, const Dropout& d, uint2 key)
+// How a token's columns are spread over its threads, kLanes threads of a
+// group at a time:
+//   MixVec     16-byte pieces; piece v's draws are one half or the whole of a
+//              group of eight elements, since a row of whole pieces starts at
+//              a multiple of its length
+//   MixLoose   any width and alignment: a warp takes 256 columns (K per lane
+//              and step, 32 apart), counted from the last multiple of eight
+//              elements before the row, so that lane l's one call of the
+//              generator gives the draws of the warp's columns 8 l .. 8 l + 7,
+//              which the lanes hand round
+template <class Elem>
+struct MixVec {
+    using Cols = VecCols<Elem>;
+    static constexpr int K = Cols::K;
+    int64_t first;  // element index of the row's start in y
+    int C, t, threads;
+
+    __device__ __forceinline__ MixVec(int64_t r, int width, int thread, int of)
+        : first(r * width), C(width), t(thread), threads(of)
+    {
+    }
+    __device__ __forceinline__ int steps() const { return (C / K + threads - 1) / threads; }
+    __device__ __forceinline__ Cols cols(int step) const
+    {
+        const int c = (step * threads + t) * K;
+        return Cols(c, c < C);
+    }
+    // Bit j: column j of `cols(step)` is kept.
+    __device__ __forceinline__ uint32_t keep(int step, const Dropout& d, uint2 key) const
+    {
+        const int64_t e = first + (step * threads + t) * K;
+        return keep_bits(e >> 3, d.offset, key, d.limit) >> (e & 7);
+    }
+};
+
+template <class Elem, int kCols>
+struct MixLoose {
+    using Cols = LooseCols<Elem, kCols>;
+    static constexpr int K = Cols::K;
+    static constexpr int kParts = 8 / K;  // steps to a warp's 256 columns
+    int64_t group;                        // of eight elements, the row's first
+    int shift, C, warp, lane, warps;
+    uint32_t bits = 0;
+
+    __device__ __forceinline__ MixLoose(int64_t r, int width, int thread, int of)
+        : group(r * width >> 3), shift(static_cast<int>(r * width & 7)), C(width), warp(thread >> 5), lane(thread & 31),
+          warps(of >> 5)
+    {
+    }
+    __device__ __forceinline__ int steps() const { return (C + shift + 256 * warps - 1) / (256 * warps) * kParts; }
+    __device__ __forceinline__ int chunk(int step) const { return (step / kParts * warps + warp) * 256; }
+    __device__ __forceinline__ Cols cols(int step) const
+    {
+        return Cols(chunk(step) + step % kParts * (32 * K) + lane - shift, 32, C);
+    }
+    // All lanes of the warp call it, step by step.
+    __device__ __forceinline__ uint32_t keep(int step, const Dropout& d, uint2 key)
+    {
+        if (step % kParts == 0) bits = keep_bits(group + (chunk(step) >> 3) + lane, d.offset, key, d.limit);
+        uint32_t k = 0;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int from = 4 * (step % kParts * K + j) + (lane >> 3);
+            k |= (__shfl_sync(0xffffffffu, bits, from) >> (lane & 7) & 1u) << j;
+        }
+        return k;
+    }
+};
+
+// y with its dropped elements at zero.
+template <int K>
+__device__ __forceinline__ void drop(float (&y)[K], uint32_t keep, float scale)
 {
-    if (!d.limit) return 1.0f;
-    return (keep_bits(e >> 3, d.offset, key, d.limit) >> (e & 7) & 1) ? d.scale : 0.0f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) y[j] = (keep >> j & 1u) ? y[j] * scale : 0.0f;
 }
 
-template <class Elem>
+// Block: (threads of a token, tokens).
+template <class Elem, class Map>
 __global__ void __launch_bounds__(kMixBlock)
-mix_fwd_rows(MixIn<Elem> in, Elem* __restrict__ out, Dropout d, int64_t N, int64_t C)
+mix_fwd_kernel(MixIn<Elem> in, Elem* __restrict__ out, Dropout d, int64_t N, int C)
 {
+    constexpr int K = Map::K;
+    const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
+    if (r >= N) return;
     const uint2 key = dropout_key(d);
-    for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-        const MixCoef k = mix_coef(in, r);
-        const Elem* x = in.x + r * in.stride;
-        for (int64_t c = threadIdx.x; c < C; c += kMixBlock) {
-            const float f = drop_factor(r * C + c, d, key);
-            const float y = f != 0.0f ? to_f32(in.y[r * in.y_stride + c]) * f : 0.0f;
-            float v[4];
+    const Elem* x = in.x + r * in.stride;
+    const Elem* yr = in.y + r * in.y_stride;
+    Elem* o = out + r * 4 * C;
+    Map map(r, C, threadIdx.x, blockDim.x);
+    const MixCoef k = mix_coef(in, r);
+    const int steps = map.steps();
+    for (int s = 0; s < steps; ++s) {
+        const typename Map::Cols cols = map.cols(s);
+        float v[4][K], y[K];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = to_f32(x[j * in.stream_stride + c]);
+        for (int j = 0; j < 4; ++j) cols.load(x + j * in.stream_stride, v[j]);
+        cols.load(yr, y);
+        if (d.limit) drop(y, map.keep(s, d, key), d.scale);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float s = k.h[i] * y;
+        for (int i = 0; i < 4; ++i) {
+            float a[K];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s = fmaf(k.t[4 * i + j], v[j], s);
-                out[(4 * r + i) * C + c] = from_f32<Elem>(s);
+            for (int c = 0; c < K; ++c) {
+                a[c] = k.h[i] * y[c];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[c] = fmaf(k.t[4 * i + j], v[j][c], a[c]);
             }
+            cols.store(o + static_cast<int64_t>(i) * C, a);
         }
     }
 }
 
-template <class Elem>
-__global__ void __launch_bounds__(kMixBlock)
-mix_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stride, MixIn<Elem> in,
-             Elem* __restrict__ dx, void* __restrict__ dT, Elem* __restrict__ dy, void* __restrict__ dh, Dropout d,
-             int64_t N, int64_t C)
+// The 20 sums of a token in one warp.  Instead of a butterfly per value, each
+// step halves the values a lane holds: it keeps one half and hands the other
+// to its partner.  Lane l ends with value `l` for l < 20 (slot order below).
+__device__ __forceinline__ float warp_sum20(const float (&a)[20])
 {
-    __shared__ float buf[20 * kMixBlock / 32];
-    const uint2 key = dropout_key(d);
-    for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-        const MixCoef k = mix_coef(in, r);
+    const int lane = threadIdx.x & 31;
+    float b[16], rest[4];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = a[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rest[i] = a[16 + i];
+    // 16 values over the lanes' bits 0..3, then bit 4: lane l has value l & 15
+#pragma unroll
+    for (int m = 8, bit = 8; m >= 1; m >>= 1, bit >>= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < m; ++i) {
+            const float give = up ? b[i] : b[i + m];
+            const float mine = up ? b[i + m] : b[i];
+            b[i] = mine + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
+    }
+    b[0] += __shfl_xor_sync(0xffffffffu, b[0], 16);
+    // 4 values over bits 0..1, then bits 2..4: lane l has value l & 3
+#pragma unroll
+    for (int m = 2, bit = 2; m >= 1; m >>= 1, bit >>= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < m; ++i) {
+            const float give = up ? rest[i] : rest[i + m];
+            const float mine = up ? rest[i + m] : rest[i];
+            rest[i] = mine + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
+    }
+#pragma unroll
+    for (int bit = 4; bit <= 16; bit <<= 1) rest[0] += __shfl_xor_sync(0xffffffffu, rest[0], bit);
+    return lane < 16 ? b[0] : rest[0];
+}
+
+template <class Elem, class Map>
+__global__ void __launch_bounds__(kMixBlock)
+mix_bwd_kernel(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stride, MixIn<Elem> in,
+               Elem* __restrict__ dx, void* __restrict__ dT, Elem* __restrict__ dy, void* __restrict__ dh, Dropout d,
+               int64_t N, int C)
+{
+    constexpr int K = Map::K;
+    __shared__ float part[kMixBlock / 32][20];
+    const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    float sum = 0.0f;
+    if (r < N) {
+        const uint2 key = dropout_key(d);
         const Elem* x = in.x + r * in.stride;
+        const Elem* yr = in.y + r * in.y_stride;
         const Elem* gr = g + r * g_stride;
+        Elem* dxr = dx + r * 4 * C;
+        Map map(r, C, threadIdx.x, blockDim.x);
+        const MixCoef k = mix_coef(in, r);
         float acc[20];
 #pragma unroll
         for (int i = 0; i < 20; ++i) acc[i] = 0.0f;
-        for (int64_t c = threadIdx.x; c < C; c += kMixBlock) {
-            const float f = drop_factor(r * C + c, d, key);
-            const float y = f != 0.0f ? to_f32(in.y[r * in.y_stride + c]) * f : 0.0f;
-            float v[4], gv[4];
+        const int steps = map.steps();
+        for (int s = 0; s < steps; ++s) {
+            const typename Map::Cols cols = map.cols(s);
+            float gv[4][K], v[4][K], y[K], b[K];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = to_f32(x[j * in.stream_stride + c]);
-                gv[j] = to_f32(gr[j * g_stream_stride + c]);
+            for (int i = 0; i < 4; ++i) cols.load(gr + i * g_stream_stride, gv[i]);
+            cols.load(yr, y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) cols.load(x + j * in.stream_stride, v[j]);
+#pragma unroll
+            for (int c = 0; c < K; ++c) {
+                b[c] = k.h[0] * gv[0][c];
+#pragma unroll
+                for (int i = 1; i < 4; ++i) b[c] = fmaf(k.h[i], gv[i][c], b[c]);
             }
-            float s = 0.0f;
+            if (d.limit) {
+                const uint32_t keep = map.keep(s, d, key);
+                drop(y, keep, d.scale);
+                drop(b, keep, d.scale);
+            }
+            cols.store(dy + r * C, b);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s = fmaf(k.h[i], gv[i], s);
-                acc[16 + i] = fmaf(gv[i], y, acc[16 + i]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[4 * i + j] = fmaf(gv[i], v[j], acc[4 * i + j]);
+                for (int c = 0; c < K; ++c) acc[16 + i] = fmaf(gv[i][c], y[c], acc[16 + i]);
             }
-            dy[r * C + c] = from_f32<Elem>(f != 0.0f ? s * f : 0.0f);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float t = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) t = fmaf(k.t[4 * i + j], gv[i], t);
-                dx[(4 * r + j) * C + c] = from_f32<Elem>(t);
+                for (int c = 0; c < K; ++c) {
+                    b[c] = k.t[j] * gv[0][c];
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) b[c] = fmaf(k.t[4 * i + j], gv[i][c], b[c]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[4 * i + j] = fmaf(gv[i][c], v[j][c], acc[4 * i + j]);
+                }
+                cols.store(dxr + static_cast<int64_t>(j) * C, b);
             }
         }
-        block_sum(acc, buf);
-        if (threadIdx.x == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) store_any(dT, 16 * r + i, in.T_dtype, acc[i]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) store_any(dh, 4 * r + i, in.h_dtype, acc[16 + i]);
-        }
-        __syncthreads();  // buf is written again
+        sum = warp_sum20(acc);
     }
+    if (warps > 1) {
+        // one token in the block: its warps' sums in warp order
+        if (lane < 20) part[threadIdx.x >> 5][lane] = sum;
+        __syncthreads();
+        if (threadIdx.x >= 32) return;
+        sum = 0.0f;
+        if (lane < 20)
+            for (int w = 0; w < warps; ++w) sum += part[w][lane];
+    }
+    if (r >= N) return;
+    if (lane < 16)
+        store_any(dT, 16 * r + lane, in.T_dtype, sum);
+    else if (lane < 20)
+        store_any(dh, 4 * r + lane - 16, in.h_dtype, sum);
 }
 
-constexpr int64_t kMaxMixGrid = int64_t{1} << 20;
+static bool aligned_streams(const void* p, int64_t stride, int64_t stream_stride, int elem)
+{
+    return aligned16(p, stride, elem) && ((stream_stride * elem) & 15) == 0;
+}
+
+template <class Elem>
+static bool mix_in_pieces(const MixIn<Elem>& in, int64_t C)
+{
+    constexpr int e = sizeof(Elem);
+    return ((C * e) & 15) == 0 && aligned_streams(in.x, in.stride, in.stream_stride, e) && aligned16(in.y, in.y_stride, e);
+}
+
+// Threads for a token of `pieces` pieces (a power of two from `least`): all
+// of them at once if a block holds them.
+static int mix_threads(int64_t pieces, int least)
+{
+    int t = least;
+    while (t < kMixBlock && t < pieces) t *= 2;
+    return t;
+}
+
+static unsigned mix_grid(int64_t N, int tokens) { return static_cast<unsigned>(ceil_div(N, tokens)); }
 
 template <class Elem>
 static int mix_forward(const MixIn<Elem>& in, void* out, const Dropout& d, int64_t N, int64_t C, cudaStream_t stream)
 {
-    mix_fwd_rows<Elem><<<static_cast<unsigned>(std::min(N, kMaxMixGrid)), kMixBlock, 0, stream>>>(
-        in, static_cast<Elem*>(out), d, N, C);
+    Elem* o = static_cast<Elem*>(out);
+    if (mix_in_pieces(in, C) && aligned16(out)) {
+        const int t = mix_threads(C / VecCols<Elem>::K, 8);
+        mix_fwd_kernel<Elem, MixVec<Elem>>
+            <<<mix_grid(N, kMixBlock / t), dim3(t, kMixBlock / t), 0, stream>>>(in, o, d, N, static_cast<int>(C));
+    } else {
+        const int t = mix_threads(ceil_div(C, 8), 32);
+        mix_fwd_kernel<Elem, MixLoose<Elem, 8>>
+            <<<mix_grid(N, kMixBlock / t), dim3(t, kMixBlock / t), 0, stream>>>(in, o, d, N, static_cast<int>(C));
+    }
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -141,9 +317,21 @@ template <class Elem>
 static int mix_backward(const void* g, int64_t g_stride, int64_t g_stream_stride, const MixIn<Elem>& in, void* dx,
                         void* dT, void* dy, void* dh, const Dropout& d, int64_t N, int64_t C, cudaStream_t stream)
 {
-    mix_bwd_rows<Elem><<<static_cast<unsigned>(std::min(N, kMaxMixGrid)), kMixBlock, 0, stream>>>(
-        static_cast<const Elem*>(g), g_stride, g_stream_stride, in, static_cast<Elem*>(dx), dT,
-        static_cast<Elem*>(dy), dh, d, N, C);
+    const Elem* gp = static_cast<const Elem*>(g);
+    Elem *dxp = static_cast<Elem*>(dx), *dyp = static_cast<Elem*>(dy);
+    const bool pieces = mix_in_pieces(in, C) && aligned_streams(g, g_stride, g_stream_stride, sizeof(Elem)) &&
+                        aligned16(dx) && aligned16(dy);
+    // A warp per token once there are tokens for every warp the GPU holds,
+    // else a block per token.
+    const int64_t per_token = pieces ? C / VecCols<Elem>::K : ceil_div(C, 8);
+    const int t = N >= 148 * 16 ? 32 : mix_threads(per_token, 32);
+    const int tokens = t == 32 ? 4 : 1;
+    if (pieces)
+        mix_bwd_kernel<Elem, MixVec<Elem>><<<mix_grid(N, tokens), dim3(t, tokens), 0, stream>>>(
+            gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, static_cast<int>(C));
+    else
+        mix_bwd_kernel<Elem, MixLoose<Elem, 4>><<<mix_grid(N, tokens), dim3(t, tokens), 0, stream>>>(
+            gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, static_cast<int>(C));
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -151,7 +339,7 @@ static bool mix_args_ok(const void* X, int64_t token_stride, int64_t stream_stri
                         int dtype, const void* T, int T_dtype, const void* h, int h_dtype, double p, int64_t N,
                         int64_t C)
 {
-    return N >= 0 && C >= 1 && token_stride >= 0 && stream_stride >= 0 && y_stride >= 0 && known_dtype(dtype) &&
+    return N >= 0 && N < (int64_t{1} << 31) && C >= 1 && C <= kMaxWidth && token_stride >= 0 && stream_stride >= 0 && y_stride >= 0 && known_dtype(dtype) &&
            known_dtype(T_dtype) && known_dtype(h_dtype) && p >= 0.0 && p <= 1.0 && (N == 0 || (X && y && T && h));
 }
 
