@@ -14,7 +14,7 @@ constexpr int kDropGroups = 4;  // groups a thread takes
 
 // A group of eight elements, one counter's draws, from and to 16-byte aligned memory.
 template <class Elem>
-struct Group {
+struct DropGroup {
     static constexpr int kPieces = 8 * sizeof(Elem) / 16;
     uint4 q[kPieces];
 
@@ -44,7 +44,7 @@ dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
     const int64_t q0 = blockIdx.x * static_cast<int64_t>(kDropBlock * kDropGroups) + threadIdx.x;
     const int64_t whole = count / 8;
     if (kVec && q0 + (kDropGroups - 1) * kDropBlock < whole) {
-        Group<Elem> g[kDropGroups];
+        DropGroup<Elem> g[kDropGroups];
 #pragma unroll
         for (int k = 0; k < kDropGroups; ++k) g[k].load(x + 8 * (q0 + k * kDropBlock));
 #pragma unroll

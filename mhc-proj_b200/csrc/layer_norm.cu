@@ -24,11 +24,37 @@ namespace mhcp {
 #ifndef MHC_RING_N
 #define MHC_RING_N 1024
 #endif
-#ifndef MHC_NORM_E16
-#define MHC_NORM_E16 1
+#ifndef MHC_SMEM
+#define MHC_SMEM 204
+#endif
+#ifndef MHC_BE
+#define MHC_BE 16
+#endif
+#ifndef MHC_BES
+#define MHC_BES 8
+#endif
+#ifndef MHC_BHS
+#define MHC_BHS true
+#endif
+#ifndef MHC_BB
+#define MHC_BB 1
+#endif
+#ifndef MHC_BBS
+#define MHC_BBS 1
+#endif
+#ifndef MHC_BT
+#define MHC_BT 2
+#endif
+#ifndef MHC_BTS
+#define MHC_BTS 1
+#endif
+#ifndef MHC_BTH
+#define MHC_BTH 512
+#endif
+#ifndef MHC_BTHS
+#define MHC_BTHS 512
 #endif
 constexpr int kNormBlock = 256;
-constexpr int kHeldThreads = 512;
 
 // One block per row, which it reads three times (the second and third come
 // from L1 or L2).
@@ -37,20 +63,23 @@ __global__ void __launch_bounds__(kNormBlock)
 norm_fwd_rows(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
               float* __restrict__ rstd_out, float eps, int64_t N, int64_t C)
 {
-    __shared__ float buf[2][kNormBlock / 32];
+    __shared__ __align__(16) float buf[2][32];
+    const Group group{kNormBlock, static_cast<int>(threadIdx.x), 0};
+    group_sum_init<1>(group, buf[0]);
+    group_sum_init<1>(group, buf[1]);
     for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
         const NormRow<Elem, kStreams> row(src, r);
         float s[1] = {0.0f};
         for (int64_t c = threadIdx.x; c < C; c += kNormBlock) s[0] += row.at(c);
-        block_sum(s, buf[0]);
+        group_sum(group, s, buf[0]);
         const float mean = s[0] / static_cast<float>(C);
         s[0] = 0.0f;
         for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
             const float d = row.at(c) - mean;
             s[0] = fmaf(d, d, s[0]);
         }
-        block_sum(s, buf[1]);
-        const float rstd = 1.0f / sqrtf(s[0] / static_cast<float>(C) + eps);
+        group_sum(group, s, buf[1]);
+        const float rstd = rsqrtf(s[0] / static_cast<float>(C) + eps);
         for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
             float v = (row.at(c) - mean) * rstd;
             if (aff.w) v *= load_any(aff.w, c, aff.dtype);
@@ -64,133 +93,17 @@ norm_fwd_rows(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__
     }
 }
 
-// The columns of a thread in a group of blockDim.x threads that hold a whole
-// row: piece p of kPieces.
-template <class Elem, bool kVec>
-struct HeldCols;
-template <class Elem>
-struct HeldCols<Elem, true> {
-    using Cols = VecCols<Elem>;
-    static __device__ __forceinline__ Cols cols(int p, int C)
-    {
-        const int c = (p * blockDim.x + threadIdx.x) * Cols::K;
-        return Cols(c, c < C);
-    }
-};
-template <class Elem>
-struct HeldCols<Elem, false> {
-    using Cols = LooseCols<Elem, 8>;
-    static __device__ __forceinline__ Cols cols(int p, int C)
-    {
-        return Cols(p * 8 * blockDim.x + threadIdx.x, blockDim.x, C);
-    }
-};
-
-// w or b at a thread's columns; `none` where there is no such array.
-template <class Elem, bool kVec, class Cols>
-__device__ __forceinline__ void load_param(const void* p, int dtype, const Cols& cols, float none, float (&v)[Cols::K])
-{
-    if (!p) {
-#pragma unroll
-        for (int j = 0; j < Cols::K; ++j) v[j] = none;
-        return;
-    }
-    if constexpr (kVec) {
-        // of x's own type, or fp32 (the launcher's rule): 16-byte pieces
-        if (sizeof(Elem) == 4 || dtype != MHC_DTYPE_F32) {
-            cols.load(static_cast<const Elem*>(p), v);
-        } else {
-            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + cols.c0);
-#pragma unroll
-            for (int i = 0; i < Cols::K / 4; ++i) {
-                const float4 f = cols.c0 >= 0 ? __ldg(q + i) : make_float4(0, 0, 0, 0);
-                v[4 * i] = f.x;
-                v[4 * i + 1] = f.y;
-                v[4 * i + 2] = f.z;
-                v[4 * i + 3] = f.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < Cols::K; ++j) v[j] = cols.has(j) ? load_any(p, cols.col(j), dtype) : none;
-    }
-}
-
-// A row held in the registers of blockDim.x threads, read once; blockDim.y
-// rows a block (more than one only where a row is one warp's).
-template <class Elem, int kStreams, bool kVec, int kElems>
-__global__ void __launch_bounds__(kHeldThreads)
-norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
-              float* __restrict__ rstd_out, float eps, int64_t N, int C)
-{
-    using Held = HeldCols<Elem, kVec>;
-    using Cols = typename Held::Cols;
-    constexpr int K = Cols::K, P = kElems / K;
-    __shared__ float buf[2][32];
-    const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
-    if (r >= N) return;
-    const NormRow<Elem, kStreams> row(src, r);
-    float u[P][K];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const Cols cols = Held::cols(p, C);
-        cols.load(row.x, u[p]);
-        if constexpr (kStreams > 1) {
-            float v[kStreams - 1][K];
-#pragma unroll
-            for (int i = 1; i < kStreams; ++i) cols.load(row.x + i * row.stream_stride, v[i - 1]);
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                u[p][j] *= row.h[0];
-#pragma unroll
-                for (int i = 1; i < kStreams; ++i) u[p][j] = fmaf(row.h[i], v[i - 1][j], u[p][j]);
-            }
-        }
-    }
-    float s[1] = {0.0f};
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int j = 0; j < K; ++j) s[0] += u[p][j];
-    }
-    block_sum(s, buf[0]);
-    const float inv = 1.0f / static_cast<float>(C), mean = s[0] * inv;
-    s[0] = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const Cols cols = Held::cols(p, C);
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            u[p][j] = cols.has(j) ? u[p][j] - mean : 0.0f;
-            s[0] = fmaf(u[p][j], u[p][j], s[0]);
-        }
-    }
-    block_sum(s, buf[1]);
-    const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const Cols cols = Held::cols(p, C);
-        float w[K], b[K];
-        load_param<Elem, kVec>(aff.w, aff.dtype, cols, 1.0f, w);
-        load_param<Elem, kVec>(aff.b, aff.dtype, cols, 0.0f, b);
-#pragma unroll
-        for (int j = 0; j < K; ++j) w[j] = fmaf(u[p][j] * rstd, w[j], b[j]);
-        cols.store(y + r * C, w);
-    }
-    if (threadIdx.x == 0) {
-        if (mean_out) mean_out[r] = mean;
-        if (rstd_out) rstd_out[r] = rstd;
-    }
-}
-
 template <class Elem, int kStreams>
 __global__ void __launch_bounds__(kNormBlock)
 norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kStreams> src,
               const float* __restrict__ mean_in, const float* __restrict__ rstd_in, NormAffine aff,
               Elem* __restrict__ dx, void* __restrict__ dh, int64_t N, int64_t C)
 {
-    __shared__ float buf[2 * kNormBlock / 32];
-    __shared__ float buf_h[4 * kNormBlock / 32];
+    __shared__ __align__(16) float buf[2 * 32];
+    __shared__ __align__(16) float buf_h[4 * 32];
+    const Group group{kNormBlock, static_cast<int>(threadIdx.x), 0};
+    group_sum_init<2>(group, buf);
+    group_sum_init<4>(group, buf_h);
     for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
         const NormRow<Elem, kStreams> row(src, r);
         const Elem* gr = g + r * g_stride;
@@ -201,7 +114,7 @@ norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kSt
             s[0] += gw;
             s[1] = fmaf(gw, (row.at(c) - mean) * rstd, s[1]);
         }
-        block_sum(s, buf);
+        group_sum(group, s, buf);
         const float m1 = s[0] / static_cast<float>(C), m2 = s[1] / static_cast<float>(C);
         float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
@@ -218,7 +131,7 @@ norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kSt
             }
         }
         if constexpr (kStreams > 1) {
-            block_sum(a, buf_h);
+            group_sum(group, a, buf_h);
             if (threadIdx.x == 0) {
 #pragma unroll
                 for (int i = 0; i < kStreams; ++i) store_any(dh, r * kStreams + i, src.h_dtype, a[i]);
@@ -264,12 +177,14 @@ norm_param_partials(const Elem* __restrict__ g, int64_t g_stride, NormSource<Ele
     }
 }
 
-// dw and db from `rows` rows of partial sums.
-__global__ void __launch_bounds__(32 * kParamRows)
+// dw and db from `rows` rows of partial sums, 32 columns a block.
+constexpr int kFoldLines = 32;
+
+__global__ void __launch_bounds__(32 * kFoldLines)
 norm_param_fold(const float* __restrict__ partials, int64_t rows, void* __restrict__ dw, void* __restrict__ db,
                 int dtype, int64_t C)
 {
-    __shared__ float part[kParamRows][32];
+    __shared__ float part[kFoldLines][33];
     const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     void* out = blockIdx.y == 0 ? dw : db;
     if (!out) return;
@@ -277,15 +192,16 @@ norm_param_fold(const float* __restrict__ partials, int64_t rows, void* __restri
         const int64_t c = c0 + lane;
         float v = 0.0f;
         if (c < C) {
-            for (int64_t k = line; k < rows; k += kParamRows) v += partials[(k * 2 + blockIdx.y) * C + c];
+#pragma unroll 8
+            for (int64_t k = line; k < rows; k += kFoldLines) v += partials[(k * 2 + blockIdx.y) * C + c];
         }
         part[line][lane] = v;
         __syncthreads();
-        if (line == 0 && c < C) {
+        // warp l folds column c0 + l
+        v = part[lane][line];
 #pragma unroll
-            for (int k = 1; k < kParamRows; ++k) v += part[k][lane];
-            store_any(out, c, dtype, v);
-        }
+        for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+        if (lane == 0 && c0 + line < C) store_any(out, c0 + line, dtype, v);
         __syncthreads();
     }
 }
@@ -313,18 +229,28 @@ static bool norm_in_pieces(const NormSource<Elem, kStreams>& src, const NormAffi
            ((!aff.w && !aff.b) || aff.dtype == own || aff.dtype == MHC_DTYPE_F32);
 }
 
-// The widest row that a block holds.
-constexpr int64_t kHeldMax = 32 * kHeldThreads;
+// Elements of a row per thread and the most threads of a block, for rows of C
+// elements: more elements as the rows get wider.
+constexpr int64_t kHeldMax = 32 * 512;
 
-template <class Elem, int kStreams, bool kVec, int kElems>
+template <class Elem, int kStreams, RowForm kForm, int kElems>
 static void norm_forward_held(const NormSource<Elem, kStreams>& src, const NormAffine& aff, Elem* y, float* mean,
                               float* rstd, float eps, int64_t N, int64_t C, cudaStream_t stream)
 {
     const int t = 32 * static_cast<int>(ceil_div(C, 32 * kElems));
     const int per_block = t == 32 ? 4 : 1;
-    norm_fwd_held<Elem, kStreams, kVec, kElems>
+    norm_fwd_held<Elem, kStreams, kForm, kElems, 512>
         <<<static_cast<unsigned>(ceil_div(N, per_block)), dim3(t, per_block), 0, stream>>>(
             src, aff, y, mean, rstd, eps, N, static_cast<int>(C));
+}
+
+// Calls `launch` with the form of the rows.
+template <class Launch>
+static cudaError_t by_form(bool pieces, bool whole, Launch launch)
+{
+    if (!pieces) return launch(std::integral_constant<RowForm, kLoose>{});
+    if (!whole) return launch(std::integral_constant<RowForm, kPieces>{});
+    return launch(std::integral_constant<RowForm, kWhole>{});
 }
 
 // The ring kernels' shape for rows of C elements.
@@ -332,17 +258,34 @@ struct RingPlan {
     int threads, groups, stages, blocks_per_sm, smem;
 };
 
-constexpr int kRingElems = 16;                // of a row, per thread
-constexpr int64_t kRingMax = 1024 * kRingElems;
-constexpr int kRingSmem = 200 * 1024;         // of an SM's 227 KB, for the ring
+// Elements of a row per thread, rows a turn and whether the parameters stay in
+// registers: rows of up to 8192 elements, and wider ones.
+template <int kStreams, bool kWide>
+struct FwdShape {
+    static constexpr int kElems = kWide ? 32 : 16, kTurn = kStreams == 1 && !kWide ? 2 : 1;
+    static constexpr bool kHold = true;
+};
+template <class Elem, int kStreams, bool kWide>
+struct BwdShape {
+    static constexpr int kNarrow = kStreams == 1 ? MHC_BE : MHC_BES;
+    static constexpr int kElems = kWide ? 2 * kNarrow : kNarrow;
+    static constexpr bool kHold = kWide ? false : kStreams == 1 ? true : MHC_BHS;
+    static constexpr int kMaxThreads = 512;
+};
+constexpr int64_t kNarrowMax = 16 * 512, kWideMax = 32 * 512;
+#ifndef MHC_MINST
+#define MHC_MINST 2
+#endif
+constexpr int kMinStages = MHC_MINST;
+constexpr int kRingSmem = MHC_SMEM * 1024;         // of an SM's 227 KB, for the ring
 
-static RingPlan ring_plan(int64_t C, int elem, bool vec, int rows, int threads_per_sm)
+static RingPlan ring_plan(int64_t C, int elem, bool vec, int rows, int per_thread, int threads_per_sm)
 {
     RingPlan p;
-    p.threads = 32 * static_cast<int>(ceil_div(C, 32 * kRingElems));
-    p.groups = p.threads == 32 ? 4 : 1;
-    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, vec, p.threads, kRingElems) * p.groups;
-    p.blocks_per_sm = std::max(1, std::min(threads_per_sm / (p.threads * p.groups), kRingSmem / (2 * stage)));
+    p.threads = 32 * static_cast<int>(ceil_div(C, 32 * per_thread));
+    p.groups = p.threads == 32 ? 8 : std::max(1, 256 / p.threads);
+    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, vec, p.threads, per_thread) * p.groups;
+    p.blocks_per_sm = std::max(1, std::min(threads_per_sm / (p.threads * p.groups), kRingSmem / (kMinStages * stage)));
     p.stages = std::min(kRingStages, std::max(1, kRingSmem / p.blocks_per_sm / stage));
     p.smem = std::max(p.stages * stage, p.groups > 1 ? static_cast<int>(8 * C) : 0);
     if (stage > 225 * 1024) p.stages = 0;  // one row does not fit
@@ -366,15 +309,16 @@ static cudaError_t allow_smem(Kernel kernel, int bytes)
                               : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <class Elem, int kStreams, bool kVec>
+template <class Elem, int kStreams, RowForm kForm, bool kWide>
 static cudaError_t norm_forward_ring(const RingPlan& p, const NormSource<Elem, kStreams>& src, const NormAffine& aff,
                                      Elem* y, float* mean, float* rstd, float eps, int64_t N, int64_t C,
                                      cudaStream_t stream)
 {
-    const auto kernel = norm_fwd_ring<Elem, kStreams, kVec, kRingElems>;
+    using S = FwdShape<kStreams, kWide>;
+    const auto kernel = norm_fwd_ring<Elem, kStreams, kForm, S::kElems, S::kTurn, S::kHold, 512>;
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
-    const int64_t grid = std::min<int64_t>(ceil_div(N, p.groups), static_cast<int64_t>(p.blocks_per_sm) * sm_count());
+    const int64_t grid = std::min<int64_t>(ceil_div(ceil_div(N, S::kTurn), p.groups), static_cast<int64_t>(p.blocks_per_sm) * sm_count());
     kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
         src, span_of(src.x, N, src.stride, kStreams, src.stream_stride, C), aff, y, mean, rstd, eps, N,
         static_cast<int>(C), p.stages);
@@ -389,23 +333,27 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, co
     const NormSource<Elem, kStreams> src{static_cast<const Elem*>(x), stride, stream_stride, h, h_dtype};
     Elem* yp = static_cast<Elem*>(y);
     const bool pieces = norm_in_pieces(src, aff, C) && aligned16(y);
-    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams, 768);
-    if (C <= kRingMax && plan.stages > 0 && N >= MHC_RING_N) {
-        const cudaError_t e = pieces ? norm_forward_ring<Elem, kStreams, true>(plan, src, aff, yp, mean, rstd, eps, N, C, stream)
-                                     : norm_forward_ring<Elem, kStreams, false>(plan, src, aff, yp, mean, rstd, eps, N, C, stream);
+    const bool wide = C > kNarrowMax;
+    const int elems = wide ? FwdShape<kStreams, true>::kElems : FwdShape<kStreams, false>::kElems;
+    const int turn = wide ? FwdShape<kStreams, true>::kTurn : FwdShape<kStreams, false>::kTurn;
+    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams * turn, elems, 512);
+    if (C <= kWideMax && plan.stages > 0 && N >= MHC_RING_N) {
+        const auto launch = [&](auto form) {
+            constexpr RowForm f = decltype(form)::value;
+            return wide ? norm_forward_ring<Elem, kStreams, f, true>(plan, src, aff, yp, mean, rstd, eps, N, C, stream)
+                        : norm_forward_ring<Elem, kStreams, f, false>(plan, src, aff, yp, mean, rstd, eps, N, C, stream);
+        };
+        const cudaError_t e = by_form(pieces, plan.threads * elems == C, launch);
         if (e != cudaSuccess) return static_cast<int>(e);
     } else if (C > kHeldMax)
         norm_fwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
             src, aff, yp, mean, rstd, eps, N, C);
-    else if (C > 16 * kHeldThreads)
-        pieces ? norm_forward_held<Elem, kStreams, true, 32>(src, aff, yp, mean, rstd, eps, N, C, stream)
-               : norm_forward_held<Elem, kStreams, false, 32>(src, aff, yp, mean, rstd, eps, N, C, stream);
-    else if (MHC_NORM_E16 || C > 8 * kHeldThreads)
-        pieces ? norm_forward_held<Elem, kStreams, true, 16>(src, aff, yp, mean, rstd, eps, N, C, stream)
-               : norm_forward_held<Elem, kStreams, false, 16>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    else if (C > 8 * 512)
+        pieces ? norm_forward_held<Elem, kStreams, kPieces, 32>(src, aff, yp, mean, rstd, eps, N, C, stream)
+               : norm_forward_held<Elem, kStreams, kLoose, 32>(src, aff, yp, mean, rstd, eps, N, C, stream);
     else
-        pieces ? norm_forward_held<Elem, kStreams, true, 8>(src, aff, yp, mean, rstd, eps, N, C, stream)
-               : norm_forward_held<Elem, kStreams, false, 8>(src, aff, yp, mean, rstd, eps, N, C, stream);
+        pieces ? norm_forward_held<Elem, kStreams, kPieces, 8>(src, aff, yp, mean, rstd, eps, N, C, stream)
+               : norm_forward_held<Elem, kStreams, kLoose, 8>(src, aff, yp, mean, rstd, eps, N, C, stream);
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -432,13 +380,14 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, in
     }
 }
 
-template <class Elem, int kStreams, bool kVec, int kMaxThreads>
+template <class Elem, int kStreams, RowForm kForm, bool kWide>
 static cudaError_t norm_backward_ring(const RingPlan& p, int64_t grid, const Elem* g, int64_t g_stride,
                                       const NormSource<Elem, kStreams>& src, const float* mean, const float* rstd,
                                       const NormAffine& aff, Elem* dx, void* dh, float* partials, int64_t N, int64_t C,
                                       cudaStream_t stream)
 {
-    const auto kernel = norm_bwd_ring<Elem, kStreams, kVec, kRingElems, kMaxThreads>;
+    using S = BwdShape<Elem, kStreams, kWide>;
+    const auto kernel = norm_bwd_ring<Elem, kStreams, kForm, S::kElems, S::kHold, S::kMaxThreads>;
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
     kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
@@ -458,20 +407,24 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
     const Elem* gp = static_cast<const Elem*>(g);
     const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
     const bool pieces = norm_in_pieces(src, aff, C) && aligned16(g, g_stride, sizeof(Elem)) && aligned16(dx);
-    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams + 1, 512);
-    if (N > 0 && C <= kRingMax && plan.stages > 0) {
-        const int64_t grid = std::min(
-            {ceil_div(N, plan.groups), static_cast<int64_t>(plan.blocks_per_sm) * sm_count(), kMaxPartials});
+    const bool wide = C > BwdShape<Elem, kStreams, false>::kElems * 512;
+    const int elems = wide ? BwdShape<Elem, kStreams, true>::kElems : BwdShape<Elem, kStreams, false>::kElems;
+    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams + 1, elems, kStreams == 1 ? MHC_BTH : MHC_BTHS);
+    if (N > 0 && plan.threads <= 512 && plan.stages > 0) {
+        const int64_t grid = std::min({ceil_div(N, plan.groups),
+                                       static_cast<int64_t>(plan.blocks_per_sm) * sm_count(), kMaxPartials});
         float* part = dw || db ? partials : nullptr;
         Elem* dxp = static_cast<Elem*>(dx);
-        const bool wide = plan.threads > 512;
-        const cudaError_t e =
-            pieces ? (wide ? norm_backward_ring<Elem, kStreams, true, 1024>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream)
-                           : norm_backward_ring<Elem, kStreams, true, 512>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream))
-                   : (wide ? norm_backward_ring<Elem, kStreams, false, 1024>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream)
-                           : norm_backward_ring<Elem, kStreams, false, 512>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp, dh, part, N, C, stream));
+        const auto launch = [&](auto form) {
+            constexpr RowForm f = decltype(form)::value;
+            return wide ? norm_backward_ring<Elem, kStreams, f, true>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp,
+                                                                      dh, part, N, C, stream)
+                        : norm_backward_ring<Elem, kStreams, f, false>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp,
+                                                                       dh, part, N, C, stream);
+        };
+        const cudaError_t e = by_form(pieces, plan.threads * elems == C, launch);
         if (e != cudaSuccess) return static_cast<int>(e);
-        if (part) norm_param_fold<<<dim3(cols, 2), 32 * kParamRows, 0, stream>>>(partials, grid, dw, db, aff.dtype, C);
+        if (part) norm_param_fold<<<dim3(cols, 2), 32 * kFoldLines, 0, stream>>>(partials, grid, dw, db, aff.dtype, C);
         return static_cast<int>(cudaGetLastError());
     }
     if (N > 0)
@@ -486,7 +439,7 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
                 <<<dim3(cols, static_cast<unsigned>(chunks)), 32 * kParamRows, 0, stream>>>(
                     gp, g_stride, src, mean, rstd, partials, N, C, chunk_rows);
         }
-        norm_param_fold<<<dim3(cols, 2), 32 * kParamRows, 0, stream>>>(partials, chunks, dw, db, aff.dtype, C);
+        norm_param_fold<<<dim3(cols, 2), 32 * kFoldLines, 0, stream>>>(partials, chunks, dw, db, aff.dtype, C);
     }
     return static_cast<int>(cudaGetLastError());
 }

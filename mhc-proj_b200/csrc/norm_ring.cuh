@@ -15,7 +15,7 @@
 #pragma once
 
 #include "norm_source.cuh"
-#include "row_ops.cuh"
+#include "row_cols.cuh"
 
 namespace mhcp {
 
@@ -62,25 +62,26 @@ __host__ __device__ inline int ring_row_bytes(int C, int elem, bool vec, int thr
 }
 
 // The ring of one group: kRows rows a stage, kElems elements of a row a thread.
-template <class Elem, int kRows, bool kVec, int kElems>
+template <class Elem, int kRows, RowForm kForm, int kElems>
 struct RowRing {
     static constexpr int kPiece = 16 / sizeof(Elem);
-    static constexpr int K = kVec ? kPiece : 8;
+    static constexpr int K = RowCols<Elem, kForm>::K;
     static constexpr int P = kElems / K;
 
     char* base;
     int row_bytes, C, t, threads;
+    RowCols<Elem, kForm> cols;
 
     __device__ __forceinline__ char* place(int stage, int row) const { return base + (stage * kRows + row) * row_bytes; }
 
     __device__ __forceinline__ void copy(int stage, int row, const Elem* from, const RowSpan& span) const
     {
         char* to = place(stage, row);
-        if constexpr (kVec) {
+        if constexpr (kForm != kLoose) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const int piece = p * threads + t;
-                if (piece * kPiece < C) copy_piece_async(to + piece * 16, from + piece * kPiece);
+                if (cols.has(p)) copy_piece_async(to + piece * 16, from + piece * kPiece);
             }
         } else {
             const char* start = reinterpret_cast<const char*>(from);
@@ -104,186 +105,217 @@ struct RowRing {
         }
     }
 
-    // Columns of piece p of this thread: col(p, j), j < K.
-    __device__ __forceinline__ int col(int p, int j) const
+    // Its 16 bytes, of rows in pieces.
+    __device__ __forceinline__ uint4 raw(int stage, int row, int p) const
     {
-        if constexpr (kVec) return (p * threads + t) * K + j;
-        return (p * K + j) * threads + t;
+        return cols.has(p) ? *reinterpret_cast<const uint4*>(place(stage, row) + (p * threads + t) * 16)
+                           : make_uint4(0, 0, 0, 0);
     }
-    __device__ __forceinline__ bool has(int p, int j) const { return col(p, kVec ? 0 : j) < C; }
 
     // Piece p of a row of a stage; `from` is where the row came from.
-    __device__ __forceinline__ void get(int stage, int row, int p, const Elem* from, float (&v)[K]) const
+    __device__ __forceinline__ void get(int stage, int row, int p, const Elem* from, float2 (&v)[K / 2]) const
     {
-        const char* at = place(stage, row);
-        if constexpr (kVec) {
-            uint4 q = make_uint4(0, 0, 0, 0);
-            if (has(p, 0)) q = *reinterpret_cast<const uint4*>(at + (p * threads + t) * 16);
-            const Elem* e = reinterpret_cast<const Elem*>(&q);
-#pragma unroll
-            for (int j = 0; j < K; ++j) v[j] = to_f32(e[j]);
+        if constexpr (kForm != kLoose) {
+            cols.unpack(raw(stage, row, p), v);
         } else {
-            const Elem* e = reinterpret_cast<const Elem*>(at + (reinterpret_cast<uintptr_t>(from) & 15));
-#pragma unroll
-            for (int j = 0; j < K; ++j) v[j] = has(p, j) ? to_f32(e[col(p, j)]) : 0.0f;
+            cols.load(p, reinterpret_cast<const Elem*>(place(stage, row) + (reinterpret_cast<uintptr_t>(from) & 15)), v);
         }
-    }
-
-    __device__ __forceinline__ void put(Elem* __restrict__ row, int p, const float (&v)[K]) const
-    {
-        if constexpr (kVec) {
-            uint4 q;
-            Elem* e = reinterpret_cast<Elem*>(&q);
-#pragma unroll
-            for (int j = 0; j < K; ++j) e[j] = from_f32<Elem>(v[j]);
-            if (has(p, 0)) *reinterpret_cast<uint4*>(row + col(p, 0)) = q;
-        } else {
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-                if (has(p, j)) row[col(p, j)] = from_f32<Elem>(v[j]);
-        }
-    }
-
-    // w or b at this thread's piece p; `none` where there is no such array.
-    __device__ __forceinline__ void param(const void* a, int dtype, int p, float none, float (&v)[K]) const
-    {
-        if (!a) {
-#pragma unroll
-            for (int j = 0; j < K; ++j) v[j] = none;
-        } else if constexpr (kVec) {
-            const Elem* own = static_cast<const Elem*>(a);
-            if (sizeof(Elem) == 4 || dtype != MHC_DTYPE_F32) {  // of the rows' own type (the launcher's rule)
-                uint4 q = make_uint4(0, 0, 0, 0);
-                if (has(p, 0)) q = __ldg(reinterpret_cast<const uint4*>(own + col(p, 0)));
-                const Elem* e = reinterpret_cast<const Elem*>(&q);
-#pragma unroll
-                for (int j = 0; j < K; ++j) v[j] = to_f32(e[j]);
-            } else {
-                const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(a) + col(p, 0));
-#pragma unroll
-                for (int i = 0; i < K / 4; ++i) {
-                    const float4 f = has(p, 0) ? __ldg(q + i) : make_float4(0, 0, 0, 0);
-                    v[4 * i] = f.x;
-                    v[4 * i + 1] = f.y;
-                    v[4 * i + 2] = f.z;
-                    v[4 * i + 3] = f.w;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < K; ++j) v[j] = has(p, j) ? load_any(a, col(p, j), dtype) : none;
-        }
-    }
-
-    // A barrier of the group.
-    __device__ __forceinline__ void sync() const
-    {
-        if (threads == 32)
-            __syncwarp();
-        else
-            __syncthreads();
     }
 };
 
 // Block: (threads of a row's group, groups); more groups than one only where a
-// group is a warp.  first + k * step are a group's rows.
-template <class Elem, int kStreams, bool kVec, int kElems>
-__global__ void __launch_bounds__(1024)
+// group is a warp.  A group takes kTurn rows at a time, next to each other, so
+// that the weight and bias are read once for them and their sums share their
+// barriers; its turns are first + k * step.
+template <class Elem, int kStreams, RowForm kForm, int kElems, int kTurn, bool kHold, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads)
 norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem* __restrict__ y,
               float* __restrict__ mean_out, float* __restrict__ rstd_out, float eps, int64_t N, int C, int stages)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ float buf[2][32];
-    using Ring = RowRing<Elem, kStreams, kVec, kElems>;
+    __shared__ __align__(16) float buf[kMaxGroups][2][kTurn * 32];
+    using Ring = RowRing<Elem, kStreams * kTurn, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
     const int threads = blockDim.x, t = threadIdx.x;
-    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kVec, threads, kElems);
-    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * kStreams * row_bytes, row_bytes, C, t, threads};
+    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm != kLoose, threads, kElems);
+    const RowCols<Elem, kForm> cols{C, t, threads};
+    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * kStreams * kTurn * row_bytes, row_bytes, C, t,
+                    threads, cols};
+    const Group group{threads, t, static_cast<int>(threadIdx.y)};
+    float(*sums)[kTurn * 32] = buf[threads > 32 ? threadIdx.y : 0];  // a warp's group needs none
+    if (threads > 32) {
+        group_sum_init<kTurn>(group, sums[0]);
+        group_sum_init<kTurn>(group, sums[1]);
+    }
+    const int64_t turns = (N + kTurn - 1) / kTurn;
     const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-    auto fill = [&](int stage, int64_t r) {
-        if (r < N) {
+    // Row q of a turn; the last turn's rows beyond the batch are its last row once more.
+    auto row_of = [&](int64_t turn, int q) { return min(turn * kTurn + q, N - 1); };
+    auto fill = [&](int stage, int64_t turn) {
+        if (turn < turns) {
 #pragma unroll
-            for (int i = 0; i < kStreams; ++i) ring.copy(stage, i, src.x + r * src.stride + i * src.stream_stride, span);
+            for (int q = 0; q < kTurn; ++q) {
+#pragma unroll
+                for (int i = 0; i < kStreams; ++i)
+                    ring.copy(stage, q * kStreams + i, src.x + row_of(turn, q) * src.stride + i * src.stream_stride, span);
+            }
         }
         copies_commit();
     };
     for (int s = 0; s < stages; ++s) fill(s, first + s * step);
     const float inv = 1.0f / static_cast<float>(C);
+    float2 held_w[kHold ? P : 1][K / 2], held_b[kHold ? P : 1][K / 2];
+    if constexpr (kHold) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            cols.param(p, aff.w, aff.dtype, 1.0f, held_w[p]);
+            cols.param(p, aff.b, aff.dtype, 0.0f, held_b[p]);
+            keep(held_w[p]);
+            keep(held_b[p]);
+        }
+    }
     int stage = 0;
-    NormRow<Elem, kStreams> next(src, min(first, N - 1));  // a row's weights are loaded one row ahead
-    for (int64_t r = first; r < N; r += step) {
-        const NormRow<Elem, kStreams> row = next;
-        next = NormRow<Elem, kStreams>(src, min(r + step, N - 1));
+    NormRow<Elem, kStreams> next[kTurn];  // rows' weights are loaded one turn ahead
+    auto look_ahead = [&](int64_t turn) {
+#pragma unroll
+        for (int q = 0; q < kTurn; ++q) next[q] = NormRow<Elem, kStreams>(src, row_of(min(turn, turns - 1), q));
+    };
+    look_ahead(first);
+    for (int64_t turn = first; turn < turns; turn += step) {
+        NormRow<Elem, kStreams> row[kTurn];
+#pragma unroll
+        for (int q = 0; q < kTurn; ++q) row[q] = next[q];
+        look_ahead(turn + step);
         copies_wait(stages);
-        if constexpr (!kVec) ring.sync();
-        float u[P][K];
-        float s[1] = {0.0f};
+        if constexpr (kForm == kLoose) group.sync();
+        float2 u[kTurn][P][K / 2];
+        float s[kTurn];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            ring.get(stage, 0, p, row.x, u[p]);
-            if constexpr (kStreams > 1) {
+        for (int q = 0; q < kTurn; ++q) {
+            float2 s2 = both(0.0f);
 #pragma unroll
-                for (int j = 0; j < K; ++j) u[p][j] *= row.h[0];
+            for (int p = 0; p < P; ++p) {
+                ring.get(stage, q * kStreams, p, row[q].x, u[q][p]);
+                if constexpr (kStreams > 1) {
 #pragma unroll
-                for (int i = 1; i < kStreams; ++i) {
-                    float v[K];
-                    ring.get(stage, i, p, row.x + i * row.stream_stride, v);
+                    for (int j = 0; j < K / 2; ++j) u[q][p][j] = mul2(u[q][p][j], both(row[q].h[0]));
 #pragma unroll
-                    for (int j = 0; j < K; ++j) u[p][j] = fmaf(row.h[i], v[j], u[p][j]);
+                    for (int i = 1; i < kStreams; ++i) {
+                        float2 v[K / 2];
+                        ring.get(stage, q * kStreams + i, p, row[q].x + i * row[q].stream_stride, v);
+#pragma unroll
+                        for (int j = 0; j < K / 2; ++j) u[q][p][j] = fma2(v[j], both(row[q].h[i]), u[q][p][j]);
+                    }
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < K; ++j) s[0] += u[p][j];
+                for (int j = 0; j < K / 2; ++j) s2 = add2(s2, u[q][p][j]);
+            }
+            s[q] = s2.x + s2.y;
         }
-        block_sum(s, buf[0]);
-        fill(stage, r + stages * step);  // all of the group have read the stage
+        group_sum(group, s, sums[0]);
+        fill(stage, turn + stages * step);  // all of the group have read the stage
         stage = stage + 1 == stages ? 0 : stage + 1;
-        const float mean = s[0] * inv;
-        s[0] = 0.0f;
+        float mean[kTurn], rstd[kTurn];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
+        for (int q = 0; q < kTurn; ++q) {
+            mean[q] = s[q] * inv;
+            float2 s2 = both(0.0f);
 #pragma unroll
-            for (int j = 0; j < K; ++j) {
-                u[p][j] = ring.has(p, j) ? u[p][j] - mean : 0.0f;
-                s[0] = fmaf(u[p][j], u[p][j], s[0]);
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int j = 0; j < K / 2; ++j) u[q][p][j] = add2(u[q][p][j], both(-mean[q]));
+                s2 = cols.squares(p, u[q][p], s2);
             }
+            s[q] = s2.x + s2.y;
         }
-        block_sum(s, buf[1]);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+        group_sum(group, s, sums[1]);
+#pragma unroll
+        for (int q = 0; q < kTurn; ++q) rstd[q] = rsqrtf(fmaf(s[q], inv, eps));
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            float w[K], b[K];
-            ring.param(aff.w, aff.dtype, p, 1.0f, w);
-            ring.param(aff.b, aff.dtype, p, 0.0f, b);
+            float2 w[K / 2], b[K / 2];
+            if constexpr (kHold) {
 #pragma unroll
-            for (int j = 0; j < K; ++j) w[j] = fmaf(u[p][j] * rstd, w[j], b[j]);
-            ring.put(y + r * C, p, w);
+                for (int j = 0; j < K / 2; ++j) {
+                    w[j] = held_w[p][j];
+                    b[j] = held_b[p][j];
+                }
+            } else {
+                cols.param(p, aff.w, aff.dtype, 1.0f, w);
+                cols.param(p, aff.b, aff.dtype, 0.0f, b);
+            }
+#pragma unroll
+            for (int q = 0; q < kTurn; ++q) {
+                float2 o[K / 2];
+#pragma unroll
+                for (int j = 0; j < K / 2; ++j) o[j] = fma2(mul2(u[q][p][j], both(rstd[q])), w[j], b[j]);
+                if (turn * kTurn + q < N) cols.store(p, y + (turn * kTurn + q) * C, o);
+            }
         }
         if (t == 0) {
-            if (mean_out) mean_out[r] = mean;
-            if (rstd_out) rstd_out[r] = rstd;
+#pragma unroll
+            for (int q = 0; q < kTurn; ++q) {
+                const int64_t r = turn * kTurn + q;
+                if (r < N && mean_out) mean_out[r] = mean[q];
+                if (r < N && rstd_out) rstd_out[r] = rstd[q];
+            }
         }
     }
 }
 
-// The backward pass, with each block's part of dw and db in registers over
-// all its rows: partials[block][0 or 1][C] (null: neither is wanted).
-template <class Elem, int kStreams, bool kVec, int kElems, int kMaxThreads>
+// Sums of 16 values over a warp: each step hands half of the values a lane
+// still holds to its partner and takes the partner's other half (16 shuffles
+// for the 16 values instead of 80).  Lane l ends with the sum of value l % 16.
+__device__ __forceinline__ float warp_sum16(float (&v)[16])
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) {
+        const bool up = lane & m;
+#pragma unroll
+        for (int i = 0; i < m; ++i) {
+            const float give = up ? v[i] : v[i + m];
+            const float mine = up ? v[i + m] : v[i];
+            v[i] = mine + __shfl_xor_sync(0xffffffffu, give, m);
+        }
+    }
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+}
+
+// The backward pass of layer norm, with each block's part of dw and db in
+// registers over all its rows: partials[block][0 or 1][C] (null: neither is
+// wanted).
+//
+// All that a row's gradients need is summed in one go over the row, so that
+// its stage is free again before the sums are known: sum(gw) and
+// sum(gw xhat), and for the streams' weights
+//   dh[i] = sum(du X[i]) = rstd (sum(gw X[i]) - m1 sum(X[i]) - m2 sum(xhat X[i])),
+// m1 = sum(gw) / C, m2 = sum(gw xhat) / C.  A thread keeps its elements' gw and
+// xhat until then (of one stream: the 16-byte pieces of g and x as they are).
+template <class Elem, int kStreams, RowForm kForm, int kElems, bool kHold, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads)
 norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, NormSource<Elem, kStreams> src,
               RowSpan span, const float* __restrict__ mean_in, const float* __restrict__ rstd_in, NormAffine aff,
               Elem* __restrict__ dx, void* __restrict__ dh, float* __restrict__ partials, int64_t N, int C, int stages)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ float buf[2][64];
-    __shared__ float buf_h[2][32 * 4];
-    using Ring = RowRing<Elem, kStreams + 1, kVec, kElems>;  // the row of g is the last of a stage
+    constexpr int kSums = kStreams == 1 ? 2 : 16;
+    __shared__ __align__(16) float buf[kMaxGroups][2][kSums * 32];
+    constexpr int kRows = kStreams + 1;  // of a stage: the streams, then g
+    using Ring = RowRing<Elem, kRows, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
     const int threads = blockDim.x, t = threadIdx.x, warps = threads >> 5;
-    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kVec, threads, kElems);
-    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * (kStreams + 1) * row_bytes, row_bytes, C, t,
-                    threads};
+    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm != kLoose, threads, kElems);
+    const RowCols<Elem, kForm> cols{C, t, threads};
+    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * kRows * row_bytes, row_bytes, C, t, threads,
+                    cols};
+    const Group group{threads, t, static_cast<int>(threadIdx.y)};
+    float(*sums)[kSums * 32] = buf[threads > 32 ? threadIdx.y : 0];  // a warp's group needs none
+    if (threads > 32) {
+        group_sum_init<2>(group, sums[0]);
+        group_sum_init<2>(group, sums[1]);
+    }
     const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
     auto fill = [&](int stage, int64_t r) {
@@ -295,22 +327,25 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
         copies_commit();
     };
     for (int s = 0; s < stages; ++s) fill(s, first + s * step);
-    float dw[P][K], db[P][K], w[P][K];
+    float2 dw[P][K / 2], db[P][K / 2], held[kHold ? P : 1][K / 2];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        ring.param(aff.w, aff.dtype, p, 1.0f, w[p]);
+        if constexpr (kHold) {
+            cols.param(p, aff.w, aff.dtype, 1.0f, held[p]);
+            keep(held[p]);
+        }
 #pragma unroll
-        for (int j = 0; j < K; ++j) dw[p][j] = db[p][j] = 0.0f;
+        for (int j = 0; j < K / 2; ++j) dw[p][j] = db[p][j] = both(0.0f);
     }
-    const float inv = 1.0f / static_cast<float>(C);
-    // dh of the group's last row: its warps' parts, put together one row later
-    auto put_dh = [&](int64_t r, int which) {
-        if (t < kStreams) {
-            float v = 0.0f;
-            for (int k = 0; k < warps; ++k) v += buf_h[which][k * 4 + t];
-            store_any(dh, r * kStreams + t, src.h_dtype, v);
+    auto weight = [&](int p, float2 (&w)[K / 2]) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int j = 0; j < K / 2; ++j) w[j] = held[p][j];
+        } else {
+            cols.param(p, aff.w, aff.dtype, 1.0f, w);
         }
     };
+    const float inv = 1.0f / static_cast<float>(C);
     int stage = 0, parity = 0;
     // a row's weights and statistics are loaded one row ahead
     int64_t ahead = min(first, N - 1);
@@ -325,97 +360,150 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
         mean_next = mean_in[ahead];
         rstd_next = rstd_in[ahead];
         copies_wait(stages);
-        if constexpr (!kVec) ring.sync();
-        // gw and xhat of a piece
-        auto piece = [&](int p, float (&gv)[K], float (&xhat)[K]) {
-            ring.get(stage, kStreams, p, gr, gv);
-            ring.get(stage, 0, p, row.x, xhat);
-            if constexpr (kStreams > 1) {
+        if constexpr (kForm == kLoose) group.sync();
+        if constexpr (kStreams == 1) {
+            // Rows in pieces are kept as they are; other rows are read from the stage twice.
+            uint4 kept[kForm != kLoose ? 2 : 1][P];
+            if constexpr (kForm != kLoose) {
 #pragma unroll
-                for (int j = 0; j < K; ++j) xhat[j] *= row.h[0];
+                for (int p = 0; p < P; ++p) {
+                    kept[0][p] = ring.raw(stage, 0, p);
+                    kept[1][p] = ring.raw(stage, 1, p);
+                }
+                fill(stage, r + stages * step);
+            }
+            auto piece = [&](int p, float2 (&gv)[K / 2], float2 (&u)[K / 2]) {
+                if constexpr (kForm != kLoose) {
+                    cols.unpack(kept[0][p], u);
+                    cols.unpack(kept[1][p], gv);
+                } else {
+                    ring.get(stage, 0, p, row.x, u);
+                    ring.get(stage, 1, p, gr, gv);
+                }
+            };
+            float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
-                for (int i = 1; i < kStreams; ++i) {
-                    float v[K];
-                    ring.get(stage, i, p, row.x + i * row.stream_stride, v);
+            for (int p = 0; p < P; ++p) {
+                float2 gv[K / 2], u[K / 2], w[K / 2];
+                piece(p, gv, u);
+                weight(p, w);
 #pragma unroll
-                    for (int j = 0; j < K; ++j) xhat[j] = fmaf(row.h[i], v[j], xhat[j]);
+                for (int j = 0; j < K / 2; ++j) {  // g is zero beyond the row
+                    const float2 xhat = mul2(add2(u[j], both(-mean)), both(rstd));
+                    const float2 gw = mul2(gv[j], w[j]);
+                    s0 = add2(s0, gw);
+                    s1 = fma2(gw, xhat, s1);
+                    dw[p][j] = fma2(gv[j], xhat, dw[p][j]);
+                    db[p][j] = add2(db[p][j], gv[j]);
                 }
             }
+            float s[2] = {s0.x + s0.y, s1.x + s1.y};
+            group_sum(group, s, sums[parity]);
+            // du = rstd (gw - m1 - (u - mean) rstd m2)
+            const float m1 = s[0] * inv, m2 = -s[1] * inv * rstd;
 #pragma unroll
-            for (int j = 0; j < K; ++j) xhat[j] = (xhat[j] - mean) * rstd;
-        };
-        float s[2] = {0.0f, 0.0f};
+            for (int p = 0; p < P; ++p) {
+                float2 du[K / 2], u[K / 2], w[K / 2];
+                piece(p, du, u);
+                weight(p, w);
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            float gv[K], xhat[K];
-            piece(p, gv, xhat);
-#pragma unroll
-            for (int j = 0; j < K; ++j) {  // g is zero beyond the row
-                dw[p][j] = fmaf(gv[j], xhat[j], dw[p][j]);
-                db[p][j] += gv[j];
-                const float gw = gv[j] * w[p][j];
-                s[0] += gw;
-                s[1] = fmaf(gw, xhat[j], s[1]);
+                for (int j = 0; j < K / 2; ++j)
+                    du[j] = mul2(both(rstd), fma2(add2(u[j], both(-mean)), both(m2), fma2(du[j], w[j], both(-m1))));
+                cols.store(p, dx + r * C, du);
             }
-        }
-        block_sum(s, buf[parity]);
-        if constexpr (kStreams > 1) {
-            if (warps > 1 && r != first) put_dh(r - step, parity ^ 1);
-        }
-        const float m1 = s[0] * inv, m2 = s[1] * inv;
-        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (kForm == kLoose) {
+                group.sync();  // others read what this thread copies over
+                fill(stage, r + stages * step);
+            }
+        } else {
+            float2 gw[P][K / 2], xhat[P][K / 2];
+            float2 s0 = both(0.0f), s1 = both(0.0f), sx[kStreams], sg[kStreams], sh[kStreams];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            float du[K], xhat[K];
-            piece(p, du, xhat);
+            for (int i = 0; i < kStreams; ++i) sx[i] = sg[i] = sh[i] = both(0.0f);
 #pragma unroll
-            for (int j = 0; j < K; ++j) du[j] = rstd * (fmaf(du[j], w[p][j], -m1) - xhat[j] * m2);
-            if constexpr (kStreams == 1) {
-                ring.put(dx + r * C, p, du);
-            } else {
+            for (int p = 0; p < P; ++p) {
+                float2 v[kStreams][K / 2], gv[K / 2], w[K / 2];
 #pragma unroll
-                for (int j = 0; j < K; ++j)
-                    if (!ring.has(p, j)) du[j] = 0.0f;
+                for (int i = 0; i < kStreams; ++i) ring.get(stage, i, p, row.x + i * row.stream_stride, v[i]);
+                ring.get(stage, kStreams, p, gr, gv);
+                weight(p, w);
 #pragma unroll
-                for (int i = 0; i < kStreams; ++i) {
-                    float v[K];
-                    ring.get(stage, i, p, row.x + i * row.stream_stride, v);
+                for (int j = 0; j < K / 2; ++j) {  // g and X are zero beyond the row
+                    float2 u = mul2(v[0][j], both(row.h[0]));
 #pragma unroll
-                    for (int j = 0; j < K; ++j) {
-                        a[i] = fmaf(du[j], v[j], a[i]);
-                        v[j] = row.h[i] * du[j];
+                    for (int i = 1; i < kStreams; ++i) u = fma2(v[i][j], both(row.h[i]), u);
+                    const float2 x = mul2(add2(u, both(-mean)), both(rstd)), y = mul2(gv[j], w[j]);
+                    s0 = add2(s0, y);
+                    s1 = fma2(y, x, s1);
+                    dw[p][j] = fma2(gv[j], x, dw[p][j]);
+                    db[p][j] = add2(db[p][j], gv[j]);
+#pragma unroll
+                    for (int i = 0; i < kStreams; ++i) {
+                        sg[i] = fma2(y, v[i][j], sg[i]);
+                        sx[i] = add2(sx[i], v[i][j]);
+                        sh[i] = fma2(x, v[i][j], sh[i]);
                     }
-                    ring.put(dx + (r * kStreams + i) * C, p, v);
+                    gw[p][j] = y;
+                    xhat[p][j] = x;
                 }
             }
-        }
-        if constexpr (kStreams > 1) {
+            if constexpr (kForm != kLoose) fill(stage, r + stages * step);
+            float all[16] = {s0.x + s0.y, s1.x + s1.y};
 #pragma unroll
             for (int i = 0; i < kStreams; ++i) {
-#pragma unroll
-                for (int m = 16; m > 0; m >>= 1) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
+                all[2 + i] = sg[i].x + sg[i].y;
+                all[6 + i] = sx[i].x + sx[i].y;
+                all[10 + i] = sh[i].x + sh[i].y;
             }
-            if (warps == 1) {
-                if (t == 0) {
-#pragma unroll
-                    for (int i = 0; i < kStreams; ++i) store_any(dh, r * kStreams + i, src.h_dtype, a[i]);
+            all[14] = all[15] = 0.0f;
+            const float mine = warp_sum16(all);
+            float m1, m2, a, b, c;  // a, b, c: of stream t, in the group's first threads
+            if (threads == 32) {
+                m1 = __shfl_sync(0xffffffffu, mine, 0);
+                m2 = __shfl_sync(0xffffffffu, mine, 1);
+                a = __shfl_sync(0xffffffffu, mine, 2 + (t & 3));
+                b = __shfl_sync(0xffffffffu, mine, 6 + (t & 3));
+                c = __shfl_sync(0xffffffffu, mine, 10 + (t & 3));
+            } else {
+                // value k of warp w at [k][w]
+                float* part = sums[parity];
+                if ((t & 31) < 14) part[(t & 31) * 32 + (t >> 5)] = mine;
+                group.sync();
+                m1 = m2 = a = b = c = 0.0f;
+                for (int k = 0; k < warps; k += 4) {  // parts of warps that the group does not have are zero
+                    const float4 f = *reinterpret_cast<const float4*>(part + k);
+                    const float4 h = *reinterpret_cast<const float4*>(part + 32 + k);
+                    m1 += (f.x + f.y) + (f.z + f.w);
+                    m2 += (h.x + h.y) + (h.z + h.w);
                 }
-            } else if ((t & 31) == 0) {
+                if (t < kStreams) {
+                    for (int k = 0; k < warps; ++k) {
+                        a += part[(2 + t) * 32 + k];
+                        b += part[(6 + t) * 32 + k];
+                        c += part[(10 + t) * 32 + k];
+                    }
+                }
+            }
+            if constexpr (kForm == kLoose) fill(stage, r + stages * step);  // all of the group have read the stage
+            m1 *= inv;
+            m2 *= inv;
+            if (t < kStreams) store_any(dh, r * kStreams + t, src.h_dtype, rstd * (a - m1 * b - m2 * c));
 #pragma unroll
-                for (int i = 0; i < kStreams; ++i) buf_h[parity][(t >> 5) * 4 + i] = a[i];
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int j = 0; j < K / 2; ++j)
+                    gw[p][j] = mul2(both(rstd), fma2(xhat[p][j], both(-m2), add2(gw[p][j], both(-m1))));
+#pragma unroll
+                for (int i = 0; i < kStreams; ++i) {
+                    float2 v[K / 2];
+#pragma unroll
+                    for (int j = 0; j < K / 2; ++j) v[j] = mul2(both(row.h[i]), gw[p][j]);
+                    cols.store(p, dx + (r * kStreams + i) * C, v);
+                }
             }
         }
-        if constexpr (!kVec) ring.sync();  // others read what this thread copies over
-        fill(stage, r + stages * step);
         stage = stage + 1 == stages ? 0 : stage + 1;
         parity ^= 1;
-    }
-    if constexpr (kStreams > 1) {
-        if (warps > 1) {
-            __syncthreads();
-            const int64_t rows = first < N ? (N - 1 - first) / step + 1 : 0;
-            if (rows > 0) put_dh(first + (rows - 1) * step, static_cast<int>((rows - 1) & 1));
-        }
     }
     if (!partials) return;
     float* out = partials + static_cast<int64_t>(blockIdx.x) * 2 * C;
@@ -429,14 +517,15 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             for (int p = 0; p < P; ++p) {
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
-                    if (!ring.has(p, j)) continue;
-                    const int c = ring.col(p, j);
+                    if (!cols.has(p, j)) continue;
+                    const int c = cols.col(p, j);
+                    float &a = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x, &b = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
                     if (k > 0) {
-                        dw[p][j] += sum[c];
-                        db[p][j] += sum[C + c];
+                        a += sum[c];
+                        b += sum[C + c];
                     }
-                    sum[c] = dw[p][j];
-                    sum[C + c] = db[p][j];
+                    sum[c] = a;
+                    sum[C + c] = b;
                 }
             }
         }
@@ -446,10 +535,83 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
     for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            if (!ring.has(p, j)) continue;
-            out[ring.col(p, j)] = dw[p][j];
-            out[C + ring.col(p, j)] = db[p][j];
+            if (!cols.has(p, j)) continue;
+            out[cols.col(p, j)] = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x;
+            out[C + cols.col(p, j)] = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
         }
+    }
+}
+
+// A row held in the registers of its group, read once and directly: for
+// batches that do not fill the GPU, where the way from the first load to the
+// last store counts.
+template <class Elem, int kStreams, RowForm kForm, int kElems, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads)
+norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
+              float* __restrict__ rstd_out, float eps, int64_t N, int C)
+{
+    using Cols = RowCols<Elem, kForm>;
+    constexpr int K = Cols::K, P = kElems / K;
+    __shared__ __align__(16) float buf[2][32];
+    const Group group{static_cast<int>(blockDim.x), static_cast<int>(threadIdx.x), 0};
+    if (blockDim.x > 32) {
+        group_sum_init<1>(group, buf[0]);
+        group_sum_init<1>(group, buf[1]);
+    }
+    const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
+    if (r >= N) return;
+    const Cols cols{C, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    const NormRow<Elem, kStreams> row(src, r);
+    float2 u[P][K / 2];
+    float2 s2 = both(0.0f);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        cols.load(p, row.x, u[p]);
+        if constexpr (kStreams > 1) {
+            float2 v[kStreams - 1][K / 2];
+#pragma unroll
+            for (int i = 1; i < kStreams; ++i) cols.load(p, row.x + i * row.stream_stride, v[i - 1]);
+#pragma unroll
+            for (int j = 0; j < K / 2; ++j) {
+                u[p][j] = mul2(u[p][j], both(row.h[0]));
+#pragma unroll
+                for (int i = 1; i < kStreams; ++i) u[p][j] = fma2(v[i - 1][j], both(row.h[i]), u[p][j]);
+            }
+        }
+    }
+    float2 w[P][K / 2], b[P][K / 2];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        cols.param(p, aff.w, aff.dtype, 1.0f, w[p]);
+        cols.param(p, aff.b, aff.dtype, 0.0f, b[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < K / 2; ++j) s2 = add2(s2, u[p][j]);
+    }
+    float s[1] = {s2.x + s2.y};
+    group_sum(group, s, buf[0]);
+    const float inv = 1.0f / static_cast<float>(C), mean = s[0] * inv;
+    s2 = both(0.0f);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < K / 2; ++j) u[p][j] = add2(u[p][j], both(-mean));
+        s2 = cols.squares(p, u[p], s2);
+    }
+    s[0] = s2.x + s2.y;
+    group_sum(group, s, buf[1]);
+    const float rstd = rsqrtf(fmaf(s[0], inv, eps));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int j = 0; j < K / 2; ++j) b[p][j] = fma2(mul2(u[p][j], both(rstd)), w[p][j], b[p][j]);
+        cols.store(p, y + r * C, b[p]);
+    }
+    if (threadIdx.x == 0) {
+        if (mean_out) mean_out[r] = mean;
+        if (rstd_out) rstd_out[r] = rstd;
     }
 }
 

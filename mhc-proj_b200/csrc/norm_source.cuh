@@ -20,6 +20,7 @@ struct NormRow {
     int64_t stream_stride;
     float h[kStreams];
 
+    NormRow() = default;
     __device__ __forceinline__ NormRow(const NormSource<Elem, kStreams>& s, int64_t r)
         : x(s.x + r * s.stride), stream_stride(s.stream_stride)
     {

@@ -1,6 +1,9 @@
 // Pieces that the row kernels (layer_norm.cu, stream_mix.cu) share.
 #pragma once
 
+#include <cstring>
+#include <type_traits>
+
 #include "mhc_common.cuh"
 #include "mhc_proj.h"
 
@@ -30,89 +33,120 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float v
     }
 }
 
-// A thread's columns of a row, K of them, as the kernels move them:
-//   VecCols     one 16-byte piece of consecutive columns.  For rows whose
-//               starts are 16-byte aligned and whose width is whole pieces.
-//   LooseCols   K columns `step` apart, one by one, so that a warp's lanes
-//               are next to each other in memory; each is in the row or not.
+// Two columns at a time: packed fp32 arithmetic, one instruction for two
+// results (the row kernels have few instruction slots per byte).
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// Holds values in registers: the compiler may otherwise load them again in
+// each turn of a loop, as it can see that they do not change.
+template <int kPairs>
+__device__ __forceinline__ void keep(float2 (&v)[kPairs])
+{
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) asm volatile("" : "+f"(v[i].x), "+f"(v[i].y));
+}
+
+// Elements 2 i and 2 i + 1 of a 16-byte piece.
 template <class Elem>
-struct VecCols {
-    static constexpr int K = 16 / sizeof(Elem);
-    int c0;  // < 0: none
-
-    __device__ __forceinline__ VecCols(int first, bool in) : c0(in ? first : -1) {}
-    __device__ __forceinline__ bool has(int) const { return c0 >= 0; }
-    __device__ __forceinline__ int col(int j) const { return c0 + j; }
-
-    __device__ __forceinline__ void load(const Elem* __restrict__ row, float (&v)[K]) const
-    {
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (c0 >= 0) q = __ldg(reinterpret_cast<const uint4*>(row + c0));
-        const Elem* e = reinterpret_cast<const Elem*>(&q);
-#pragma unroll
-        for (int j = 0; j < K; ++j) v[j] = to_f32(e[j]);
+__device__ __forceinline__ float2 pair_of(const uint4& q, int i)
+{
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(Elem) == 4) {
+        return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    } else if constexpr (std::is_same<Elem, __nv_bfloat16>::value) {
+        return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    } else {
+        __half2 h;
+        memcpy(&h, &w[i], 4);
+        return __half22float2(h);
     }
+}
 
-    __device__ __forceinline__ void store(Elem* __restrict__ row, const float (&v)[K]) const
-    {
-        uint4 q;
-        Elem* e = reinterpret_cast<Elem*>(&q);
+// The 16-byte piece of K elements.
+template <class Elem, int kPairs>
+__device__ __forceinline__ uint4 piece_of(const float2 (&v)[kPairs])
+{
+    unsigned w[4];
 #pragma unroll
-        for (int j = 0; j < K; ++j) e[j] = from_f32<Elem>(v[j]);
-        if (c0 >= 0) *reinterpret_cast<uint4*>(row + c0) = q;
+    for (int i = 0; i < kPairs; ++i) {
+        if constexpr (sizeof(Elem) == 4) {
+            w[2 * i] = __float_as_uint(v[i].x);
+            w[2 * i + 1] = __float_as_uint(v[i].y);
+        } else if constexpr (std::is_same<Elem, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+            memcpy(&w[i], &h, 4);
+        } else {
+            const __half2 h = __float22half2_rn(v[i]);
+            memcpy(&w[i], &h, 4);
+        }
     }
-};
-
-template <class Elem, int kCols>
-struct LooseCols {
-    static constexpr int K = kCols;
-    int c0, step, C;
-
-    __device__ __forceinline__ LooseCols(int first, int stride, int width) : c0(first), step(stride), C(width) {}
-    __device__ __forceinline__ int col(int j) const { return c0 + j * step; }
-    __device__ __forceinline__ bool has(int j) const { return static_cast<unsigned>(col(j)) < static_cast<unsigned>(C); }
-
-    __device__ __forceinline__ void load(const Elem* __restrict__ row, float (&v)[K]) const
-    {
-#pragma unroll
-        for (int j = 0; j < K; ++j) v[j] = has(j) ? to_f32(row[col(j)]) : 0.0f;
-    }
-
-    __device__ __forceinline__ void store(Elem* __restrict__ row, const float (&v)[K]) const
-    {
-#pragma unroll
-        for (int j = 0; j < K; ++j)
-            if (has(j)) row[col(j)] = from_f32<Elem>(v[j]);
-    }
-};
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Widths are ints in the kernels.
 constexpr int64_t kMaxWidth = int64_t{1} << 30;
 
-// Sums of K values over the block's threads, in every thread, in an order
-// fixed by the block's size.  `buf` holds K floats per warp; the caller keeps
-// two calls with the same buf apart (by a barrier or by alternating buffers).
+// The threads that work on one row: a warp, or several warps of a block, which
+// may hold other groups (each has a barrier of its own).
+struct Group {
+    int threads, t, id;
+
+    __device__ __forceinline__ void sync() const
+    {
+        if (threads == 32)
+            __syncwarp();
+        else if (blockDim.y == 1)
+            __syncthreads();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+    }
+};
+
+constexpr int kMaxGroups = 4;  // of more than a warp, in a block
+
+// Sums of K values over a group's threads, in every thread, in an order fixed
+// by the group's size.  `buf`: 32 K floats of the group at a 16-byte boundary
+// that group_sum_init has seen; the caller keeps two calls with the same buf
+// apart (by a barrier or by alternating buffers).
 template <int K>
-__device__ __forceinline__ void block_sum(float (&v)[K], float* buf)
+__device__ __forceinline__ void group_sum_init(const Group& g, float* buf)
+{
+    // parts of warps that the group does not have: added as zeros
+    if (g.t >= g.threads >> 5 && g.t < 32) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) buf[k * 32 + g.t] = 0.0f;
+    }
+}
+
+template <int K>
+__device__ __forceinline__ void group_sum(const Group& g, float (&v)[K], float* buf)
 {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int m = 16; m > 0; m >>= 1) {
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
     }
-    const int warps = blockDim.x >> 5;
-    if (warps == 1) return;
-    if ((threadIdx.x & 31) == 0) {
+    if (g.threads == 32) return;
+    if ((g.t & 31) == 0) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) buf[(threadIdx.x >> 5) * K + k] = v[k];
+        for (int k = 0; k < K; ++k) buf[k * 32 + (g.t >> 5)] = v[k];
     }
-    __syncthreads();
+    g.sync();
+    float4 f[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = buf[k];
-    for (int w = 1; w < warps; ++w) {
+    for (int k = 0; k < K; ++k) f[k] = *reinterpret_cast<const float4*>(buf + k * 32);
+    for (int w = 4; w < g.threads >> 5; w += 4) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += buf[w * K + k];
+        for (int k = 0; k < K; ++k) {
+            const float4 o = *reinterpret_cast<const float4*>(buf + k * 32 + w);
+            f[k] = make_float4(f[k].x + o.x, f[k].y + o.y, f[k].z + o.z, f[k].w + o.w);
+        }
     }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = (f[k].x + f[k].y) + (f[k].z + f[k].w);
 }
 
 }  // namespace mhcp

@@ -15,6 +15,9 @@
 
 namespace mhcp {
 
+#ifndef MHC_MIXF_T
+#define MHC_MIXF_T 256
+#endif
 constexpr int kMixBlock = 256;
 
 template <class Elem>
@@ -43,6 +46,62 @@ __device__ __forceinline__ MixCoef mix_coef(const MixIn<Elem>& in, int64_t r)
     return k;
 }
 
+// A thread's columns of a row, K of them, as the kernels move them:
+//   MixVecCols     one 16-byte piece of consecutive columns.  For rows whose
+//               starts are 16-byte aligned and whose width is whole pieces.
+//   MixLooseCols   K columns `step` apart, one by one, so that a warp's lanes
+//               are next to each other in memory; each is in the row or not.
+template <class Elem>
+struct MixVecCols {
+    static constexpr int K = 16 / sizeof(Elem);
+    int c0;  // < 0: none
+
+    __device__ __forceinline__ MixVecCols(int first, bool in) : c0(in ? first : -1) {}
+    __device__ __forceinline__ bool has(int) const { return c0 >= 0; }
+    __device__ __forceinline__ int col(int j) const { return c0 + j; }
+
+    __device__ __forceinline__ void load(const Elem* __restrict__ row, float (&v)[K]) const
+    {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (c0 >= 0) q = __ldg(reinterpret_cast<const uint4*>(row + c0));
+        const Elem* e = reinterpret_cast<const Elem*>(&q);
+#pragma unroll
+        for (int j = 0; j < K; ++j) v[j] = to_f32(e[j]);
+    }
+
+    __device__ __forceinline__ void store(Elem* __restrict__ row, const float (&v)[K]) const
+    {
+        uint4 q;
+        Elem* e = reinterpret_cast<Elem*>(&q);
+#pragma unroll
+        for (int j = 0; j < K; ++j) e[j] = from_f32<Elem>(v[j]);
+        if (c0 >= 0) *reinterpret_cast<uint4*>(row + c0) = q;
+    }
+};
+
+template <class Elem, int kCols>
+struct MixLooseCols {
+    static constexpr int K = kCols;
+    int c0, step, C;
+
+    __device__ __forceinline__ MixLooseCols(int first, int stride, int width) : c0(first), step(stride), C(width) {}
+    __device__ __forceinline__ int col(int j) const { return c0 + j * step; }
+    __device__ __forceinline__ bool has(int j) const { return static_cast<unsigned>(col(j)) < static_cast<unsigned>(C); }
+
+    __device__ __forceinline__ void load(const Elem* __restrict__ row, float (&v)[K]) const
+    {
+#pragma unroll
+        for (int j = 0; j < K; ++j) v[j] = has(j) ? to_f32(row[col(j)]) : 0.0f;
+    }
+
+    __device__ __forceinline__ void store(Elem* __restrict__ row, const float (&v)[K]) const
+    {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            if (has(j)) row[col(j)] = from_f32<Elem>(v[j]);
+    }
+};
+
 // How a token's columns are spread over its threads, kLanes threads of a
 // group at a time:
 //   MixVec     16-byte pieces; piece v's draws are one half or the whole of a
@@ -55,7 +114,7 @@ __device__ __forceinline__ MixCoef mix_coef(const MixIn<Elem>& in, int64_t r)
 //              which the lanes hand round
 template <class Elem>
 struct MixVec {
-    using Cols = VecCols<Elem>;
+    using Cols = MixVecCols<Elem>;
     static constexpr int K = Cols::K;
     int64_t first;  // element index of the row's start in y
     int C, t, threads;
@@ -80,7 +139,7 @@ struct MixVec {
 
 template <class Elem, int kCols>
 struct MixLoose {
-    using Cols = LooseCols<Elem, kCols>;
+    using Cols = MixLooseCols<Elem, kCols>;
     static constexpr int K = Cols::K;
     static constexpr int kParts = 8 / K;  // steps to a warp's 256 columns
     int64_t group;                        // of eight elements, the row's first
@@ -302,7 +361,8 @@ static int mix_forward(const MixIn<Elem>& in, void* out, const Dropout& d, int64
 {
     Elem* o = static_cast<Elem*>(out);
     if (mix_in_pieces(in, C) && aligned16(out)) {
-        const int t = mix_threads(C / VecCols<Elem>::K, 8);
+        int t = mix_threads(C / MixVecCols<Elem>::K, 8);
+        if (N >= 148 * 16) t = std::min(t, MHC_MIXF_T);
         mix_fwd_kernel<Elem, MixVec<Elem>>
             <<<mix_grid(N, kMixBlock / t), dim3(t, kMixBlock / t), 0, stream>>>(in, o, d, N, static_cast<int>(C));
     } else {
@@ -323,7 +383,7 @@ static int mix_backward(const void* g, int64_t g_stride, int64_t g_stream_stride
                         aligned16(dx) && aligned16(dy);
     // A warp per token once there are tokens for every warp the GPU holds,
     // else a block per token.
-    const int64_t per_token = pieces ? C / VecCols<Elem>::K : ceil_div(C, 8);
+    const int64_t per_token = pieces ? C / MixVecCols<Elem>::K : ceil_div(C, 8);
     const int t = N >= 148 * 16 ? 32 : mix_threads(per_token, 32);
     const int tokens = t == 32 ? 4 : 1;
     if (pieces)
