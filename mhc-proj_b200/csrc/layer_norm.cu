@@ -17,7 +17,7 @@
 
 #include "norm_ring.cuh"
 #include "norm_source.cuh"
-#include "row_ops.cuh"
+#include "row_copy.cuh"
 
 namespace mhcp {
 
@@ -290,23 +290,6 @@ static RingPlan ring_plan(int64_t C, int elem, bool vec, int rows, int per_threa
     p.smem = std::max(p.stages * stage, p.groups > 1 ? static_cast<int>(8 * C) : 0);
     if (stage > 225 * 1024) p.stages = 0;  // one row does not fit
     return p;
-}
-
-static int sm_count()
-{
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return 0;
-    return sms;
-}
-
-// A launch may need more dynamic shared memory than a kernel has by default;
-// the attribute belongs to the context, so it is set for each such launch.
-template <class Kernel>
-static cudaError_t allow_smem(Kernel kernel, int bytes)
-{
-    return bytes <= 44 * 1024 ? cudaSuccess  // 48 KB less what is static
-                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 template <class Elem, int kStreams, RowForm kForm, bool kWide>

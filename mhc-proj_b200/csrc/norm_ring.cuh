@@ -16,44 +16,9 @@
 
 #include "norm_source.cuh"
 #include "row_cols.cuh"
+#include "row_copy.cuh"
 
 namespace mhcp {
-
-__device__ __forceinline__ void copy_piece_async(void* smem, const void* global)
-{
-    const unsigned s = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(global) : "memory");
-}
-
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-
-// Waits until at most `stages` - 1 of this thread's batches of copies are under way.
-__device__ __forceinline__ void copies_wait(int stages)
-{
-    if (stages >= 4)
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (stages == 3)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (stages == 2)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
-
-constexpr int kRingStages = 4;  // at most
-
-// A tensor of rows: the row's address is base + r * stride, and [lo, hi) are
-// the bytes from its first to its last element.
-struct RowSpan {
-    const char *lo, *hi;
-};
-
-template <class Elem>
-inline RowSpan span_of(const Elem* p, int64_t N, int64_t stride, int streams, int64_t stream_stride, int64_t C)
-{
-    return {reinterpret_cast<const char*>(p),
-            reinterpret_cast<const char*>(p + (N - 1) * stride + (streams - 1) * stream_stride + C)};
-}
 
 // Bytes of one row's place in a stage.
 __host__ __device__ inline int ring_row_bytes(int C, int elem, bool vec, int threads, int per_thread)
@@ -74,7 +39,8 @@ struct RowRing {
 
     __device__ __forceinline__ char* place(int stage, int row) const { return base + (stage * kRows + row) * row_bytes; }
 
-    __device__ __forceinline__ void copy(int stage, int row, const Elem* from, const RowSpan& span) const
+    // amid: the tensor has 32 bytes on both sides of the row
+    __device__ __forceinline__ void copy(int stage, int row, const Elem* from, const RowSpan& span, bool amid) const
     {
         char* to = place(stage, row);
         if constexpr (kForm != kLoose) {
@@ -84,28 +50,18 @@ struct RowRing {
                 if (cols.has(p)) copy_piece_async(to + piece * 16, from + piece * kPiece);
             }
         } else {
-            const char* start = reinterpret_cast<const char*>(from);
-            const char* end = reinterpret_cast<const char*>(from + C);
-            const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(start) & 15);
-            const char* first = start - shift;
-            const int pieces = (shift + C * static_cast<int>(sizeof(Elem)) + 15) >> 4;
-            for (int q = t; q < pieces; q += threads) {
-                const char* src = first + 16 * q;
-                if (src >= span.lo && src + 16 <= span.hi) {
-                    copy_piece_async(to + 16 * q, src);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kPiece; ++i) {
-                        const char* e = src + i * sizeof(Elem);
-                        if (e >= start && e < end)
-                            reinterpret_cast<Elem*>(to + 16 * q)[i] = *reinterpret_cast<const Elem*>(e);
-                    }
-                }
+            const int skew = offset_in_piece(from);
+            const int pieces = (skew + C * static_cast<int>(sizeof(Elem)) + 15) >> 4;
+            const char* src = reinterpret_cast<const char*>(from) - skew;
+            if (amid) {
+                for (int q = t; q < pieces; q += threads) copy_piece_async(to + 16 * q, src + 16 * q);
+            } else {
+                for (int q = t; q < pieces; q += threads) copy_checked_piece(to + 16 * q, src + 16 * q, from, from + C, span);
             }
         }
     }
 
-    // Its 16 bytes, of rows in pieces.
+    // The 16 bytes of piece p of a row of a stage, of rows in pieces.
     __device__ __forceinline__ uint4 raw(int stage, int row, int p) const
     {
         return cols.has(p) ? *reinterpret_cast<const uint4*>(place(stage, row) + (p * threads + t) * 16)
@@ -118,7 +74,7 @@ struct RowRing {
         if constexpr (kForm != kLoose) {
             cols.unpack(raw(stage, row, p), v);
         } else {
-            cols.load(p, reinterpret_cast<const Elem*>(place(stage, row) + (reinterpret_cast<uintptr_t>(from) & 15)), v);
+            cols.load(p, reinterpret_cast<const Elem*>(place(stage, row) + offset_in_piece(from)), v);
         }
     }
 };
@@ -158,7 +114,8 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
             for (int q = 0; q < kTurn; ++q) {
 #pragma unroll
                 for (int i = 0; i < kStreams; ++i)
-                    ring.copy(stage, q * kStreams + i, src.x + row_of(turn, q) * src.stride + i * src.stream_stride, span);
+                    ring.copy(stage, q * kStreams + i, src.x + row_of(turn, q) * src.stride + i * src.stream_stride, span,
+                              span.amid(row_of(turn, q), N));
             }
         }
         copies_commit();
@@ -321,8 +278,8 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
     auto fill = [&](int stage, int64_t r) {
         if (r < N) {
 #pragma unroll
-            for (int i = 0; i < kStreams; ++i) ring.copy(stage, i, src.x + r * src.stride + i * src.stream_stride, span);
-            ring.copy(stage, kStreams, g + r * g_stride, g_span);
+            for (int i = 0; i < kStreams; ++i) ring.copy(stage, i, src.x + r * src.stride + i * src.stream_stride, span, span.amid(r, N));
+            ring.copy(stage, kStreams, g + r * g_stride, g_span, g_span.amid(r, N));
         }
         copies_commit();
     };

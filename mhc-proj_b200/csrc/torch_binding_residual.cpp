@@ -9,6 +9,8 @@
 // move to its device.
 #include <optional>
 
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "torch_binding.h"
 
 namespace mhcp_torch {
@@ -58,10 +60,33 @@ torch::TensorOptions compute_options(const torch::Tensor& x, std::initializer_li
     return opts.dtype(x.scalar_type());
 }
 
+// x of opts' device and type.  A call on a few tokens takes little longer than
+// its trips through the dispatcher, so nothing is asked of it that is so already.
+torch::Tensor on(const torch::Tensor& x, const torch::TensorOptions& opts)
+{
+    return x.device() == opts.device() && x.scalar_type() == opts.dtype() ? x : x.to(opts);
+}
+
+torch::Tensor whole(const torch::Tensor& x) { return x.is_contiguous() ? x : x.contiguous(); }
+
+// An uninitialised contiguous tensor of opts' device.
+torch::Tensor fresh(at::IntArrayRef sizes, const torch::TensorOptions& opts, torch::ScalarType type)
+{
+    return at::detail::empty_cuda(sizes, type, opts.device(), std::nullopt);
+}
+
+torch::Tensor fresh(at::IntArrayRef sizes, const torch::TensorOptions& opts)
+{
+    return fresh(sizes, opts, c10::typeMetaToScalarType(opts.dtype()));
+}
+
+// A result in the type and on the device that the caller's tensor has.
+torch::Tensor as(const torch::Tensor& x, const torch::TensorOptions& src) { return on(x, src); }
+
 // x on opts with its last dimension contiguous (a copy only where needed).
 torch::Tensor rows_on(const torch::Tensor& x, const torch::TensorOptions& opts)
 {
-    torch::Tensor t = x.to(opts);
+    torch::Tensor t = on(x, opts);
     return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
@@ -69,7 +94,7 @@ torch::Tensor rows_on(const torch::Tensor& x, const torch::TensorOptions& opts)
 // own type when the kernels take it, else fp32.
 torch::Tensor small_on(const torch::Tensor& x, const torch::TensorOptions& opts)
 {
-    return x.to(dtype_code(x) >= 0 ? opts.dtype(x.scalar_type()) : opts.dtype(torch::kFloat32)).contiguous();
+    return whole(on(x, opts.dtype(dtype_code(x) >= 0 ? x.scalar_type() : torch::kFloat32)));
 }
 
 void check_affine(const Opt& weight, const Opt& bias, int64_t width)
@@ -102,7 +127,7 @@ struct Affine {
     const void* weight() const { return w.defined() ? w.data_ptr() : nullptr; }
     const void* bias() const { return b.defined() ? b.data_ptr() : nullptr; }
     // Somewhere to write the gradient of a given parameter, in the pair's type.
-    torch::Tensor grad_of(const torch::Tensor& of) const { return of.defined() ? torch::empty_like(of) : torch::Tensor(); }
+    torch::Tensor grad_of(const torch::Tensor& of) const { return of.defined() ? fresh(of.sizes(), of.options()) : torch::Tensor(); }
 };
 
 void* ptr(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -124,14 +149,14 @@ py::dict layer_norm(torch::Tensor x, const Opt& weight, const Opt& bias, double 
     const Affine a(weight, bias, opts);
     x = rows_on(x, opts);
     const c10::cuda::CUDAGuard guard(x.device());
-    torch::Tensor y = torch::empty({n, c}, opts);
-    torch::Tensor mean = torch::empty({n}, opts.dtype(torch::kFloat32)), rstd = torch::empty_like(mean);
+    torch::Tensor y = fresh({n, c}, opts);
+    torch::Tensor mean = fresh({n}, opts, torch::kFloat32), rstd = fresh({n}, opts, torch::kFloat32);
     check_status(mhc_layer_norm(x.data_ptr(), x.stride(0), dtype_code(x), a.weight(), a.bias(), a.dtype, y.data_ptr(),
                                 mean.data_ptr<float>(), rstd.data_ptr<float>(), static_cast<float>(eps), n, c,
                                 current_stream()),
                  "layer_norm");
     py::dict out;
-    out["y"] = y.to(src);
+    out["y"] = as(y, src);
     out["mean"] = mean;
     out["rstd"] = rstd;
     return out;
@@ -146,14 +171,14 @@ void check_stats(const torch::Tensor& mean, const torch::Tensor& rstd, int64_t n
 
 torch::Tensor stats_on(const torch::Tensor& s, const torch::TensorOptions& opts)
 {
-    return s.to(opts.dtype(torch::kFloat32)).contiguous();
+    return whole(on(s, opts.dtype(torch::kFloat32)));
 }
 
 void put_affine_grads(py::dict& out, const torch::Tensor& dw, const torch::Tensor& db, const Opt& weight,
                       const Opt& bias)
 {
-    if (weight) out["d_weight"] = dw.to(weight->options());
-    if (bias) out["d_bias"] = db.to(bias->options());
+    if (weight) out["d_weight"] = as(dw, weight->options());
+    if (bias) out["d_bias"] = as(db, bias->options());
 }
 
 py::dict layer_norm_backward(torch::Tensor G, torch::Tensor x, torch::Tensor mean, torch::Tensor rstd,
@@ -174,19 +199,19 @@ py::dict layer_norm_backward(torch::Tensor G, torch::Tensor x, torch::Tensor mea
     x = rows_on(x, opts);
     G = rows_on(G, opts);
     const c10::cuda::CUDAGuard guard(x.device());
-    torch::Tensor dx = torch::empty({n, c}, opts);
+    torch::Tensor dx = fresh({n, c}, opts);
     torch::Tensor dw = a.grad_of(a.w), db = a.grad_of(a.b), ws;
     int64_t bytes = 0;
     if (weight || bias) {
         check_status(mhc_layer_norm_backward_workspace(n, c, &bytes), "layer_norm_backward");
-        ws = torch::empty({bytes}, opts.dtype(torch::kUInt8));
+        ws = fresh({bytes}, opts, torch::kUInt8);
     }
     check_status(mhc_layer_norm_backward(G.data_ptr(), G.stride(0), x.data_ptr(), x.stride(0), dtype_code(x),
                                          mean.data_ptr<float>(), rstd.data_ptr<float>(), a.weight(), a.dtype,
                                          dx.data_ptr(), ptr(dw), ptr(db), n, c, ptr(ws), bytes, current_stream()),
                  "layer_norm_backward");
     py::dict out;
-    out["d_x"] = dx.to(src);
+    out["d_x"] = as(dx, src);
     put_affine_grads(out, dw, db, weight, bias);
     return out;
 }
@@ -232,13 +257,13 @@ torch::Tensor dropped(torch::Tensor x, double p, const py::object& seed, int64_t
     const auto src = x.options();
     const auto opts = compute_options(x);
     const Seed key(seed, opts);
-    x = x.to(opts).contiguous();
+    x = whole(on(x, opts));
     const c10::cuda::CUDAGuard guard(x.device());
-    torch::Tensor y = torch::empty(x.sizes(), opts);
+    torch::Tensor y = fresh(x.sizes(), opts);
     check_status(mhc_dropout(x.data_ptr(), y.data_ptr(), dtype_code(x), x.numel(), p, key.value, key.device(), offset,
                              current_stream()),
                  what);
-    return y.to(src);
+    return as(y, src);
 }
 
 py::dict dropout(torch::Tensor x, double p, py::object seed, int64_t offset)
@@ -270,14 +295,14 @@ py::dict stream_norm_n4(torch::Tensor X, torch::Tensor h_pre, const Opt& weight,
     X = rows_on(X, opts);
     const torch::Tensor h = small_on(h_pre, opts);
     const c10::cuda::CUDAGuard guard(X.device());
-    torch::Tensor y = torch::empty({n, c}, opts);
-    torch::Tensor mean = torch::empty({n}, opts.dtype(torch::kFloat32)), rstd = torch::empty_like(mean);
+    torch::Tensor y = fresh({n, c}, opts);
+    torch::Tensor mean = fresh({n}, opts, torch::kFloat32), rstd = fresh({n}, opts, torch::kFloat32);
     check_status(mhc_stream_norm_n4(X.data_ptr(), X.stride(0), X.stride(1), dtype_code(X), h.data_ptr(), dtype_code(h),
                                     a.weight(), a.bias(), a.dtype, y.data_ptr(), mean.data_ptr<float>(),
                                     rstd.data_ptr<float>(), static_cast<float>(eps), n, c, current_stream()),
                  "stream_norm_n4");
     py::dict out;
-    out["y"] = y.to(src);
+    out["y"] = as(y, src);
     out["mean"] = mean;
     out["rstd"] = rstd;
     return out;
@@ -304,13 +329,13 @@ py::dict stream_norm_n4_backward(torch::Tensor G, torch::Tensor X, torch::Tensor
     G = rows_on(G, opts);
     const torch::Tensor h = small_on(h_pre, opts);
     const c10::cuda::CUDAGuard guard(X.device());
-    torch::Tensor dX = torch::empty({n, 4, c}, opts);
-    torch::Tensor dh = torch::empty_like(h);
+    torch::Tensor dX = fresh({n, 4, c}, opts);
+    torch::Tensor dh = fresh(h.sizes(), h.options());
     torch::Tensor dw = a.grad_of(a.w), db = a.grad_of(a.b), ws;
     int64_t bytes = 0;
     if (weight || bias) {
         check_status(mhc_stream_norm_n4_backward_workspace(n, c, &bytes), "stream_norm_n4_backward");
-        ws = torch::empty({bytes}, opts.dtype(torch::kUInt8));
+        ws = fresh({bytes}, opts, torch::kUInt8);
     }
     check_status(mhc_stream_norm_n4_backward(G.data_ptr(), G.stride(0), X.data_ptr(), X.stride(0), X.stride(1),
                                              dtype_code(X), h.data_ptr(), dtype_code(h), mean.data_ptr<float>(),
@@ -318,8 +343,8 @@ py::dict stream_norm_n4_backward(torch::Tensor G, torch::Tensor X, torch::Tensor
                                              ptr(dw), ptr(db), n, c, ptr(ws), bytes, current_stream()),
                  "stream_norm_n4_backward");
     py::dict out;
-    out["d_X"] = dX.to(src);
-    out["d_h_pre"] = dh.to(h_pre.options());
+    out["d_X"] = as(dX, src);
+    out["d_h_pre"] = as(dh, h_pre.options());
     put_affine_grads(out, dw, db, weight, bias);
     return out;
 }
@@ -352,13 +377,13 @@ py::dict stream_mix_n4(torch::Tensor X, torch::Tensor T, torch::Tensor y, torch:
     y = rows_on(y, opts);
     const torch::Tensor t = small_on(T, opts), h = small_on(h_post, opts);
     const c10::cuda::CUDAGuard guard(X.device());
-    torch::Tensor out_x = torch::empty({n, 4, c}, opts);
+    torch::Tensor out_x = fresh({n, 4, c}, opts);
     check_status(mhc_stream_mix_n4(X.data_ptr(), X.stride(0), X.stride(1), y.data_ptr(), y.stride(0), dtype_code(X),
                                    t.data_ptr(), dtype_code(t), h.data_ptr(), dtype_code(h), out_x.data_ptr(), p,
                                    key.value, key.device(), offset, n, c, current_stream()),
                  "stream_mix_n4");
     py::dict out;
-    out["X"] = out_x.to(src);
+    out["X"] = as(out_x, src);
     return out;
 }
 
@@ -377,8 +402,8 @@ py::dict stream_mix_n4_backward(torch::Tensor G, torch::Tensor X, torch::Tensor 
     G = rows_on(G, opts);
     const torch::Tensor t = small_on(T, opts), h = small_on(h_post, opts);
     const c10::cuda::CUDAGuard guard(X.device());
-    torch::Tensor dX = torch::empty({n, 4, c}, opts), dT = torch::empty_like(t);
-    torch::Tensor dy = torch::empty({n, c}, opts), dh = torch::empty_like(h);
+    torch::Tensor dX = fresh({n, 4, c}, opts), dT = fresh(t.sizes(), t.options());
+    torch::Tensor dy = fresh({n, c}, opts), dh = fresh(h.sizes(), h.options());
     check_status(mhc_stream_mix_n4_backward(G.data_ptr(), G.stride(0), G.stride(1), X.data_ptr(), X.stride(0),
                                             X.stride(1), y.data_ptr(), y.stride(0), dtype_code(X), t.data_ptr(),
                                             dtype_code(t), h.data_ptr(), dtype_code(h), dX.data_ptr(), dT.data_ptr(),
@@ -386,10 +411,10 @@ py::dict stream_mix_n4_backward(torch::Tensor G, torch::Tensor X, torch::Tensor 
                                             current_stream()),
                  "stream_mix_n4_backward");
     py::dict out;
-    out["d_X"] = dX.to(src);
-    out["d_T"] = dT.to(T.options());
-    out["d_y"] = dy.to(y_src);
-    out["d_h_post"] = dh.to(h_post.options());
+    out["d_X"] = as(dX, src);
+    out["d_T"] = as(dT, T.options());
+    out["d_y"] = as(dy, y_src);
+    out["d_h_post"] = as(dh, h_post.options());
     return out;
 }
 
