@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "norm_ring.cuh"
+#include "norm_rows.cuh"
 #include "norm_source.cuh"
 #include "row_copy.cuh"
 
@@ -24,187 +25,6 @@ namespace mhcp {
 #ifndef MHC_RING_N
 #define MHC_RING_N 1024
 #endif
-#ifndef MHC_SMEM
-#define MHC_SMEM 204
-#endif
-#ifndef MHC_BE
-#define MHC_BE 16
-#endif
-#ifndef MHC_BES
-#define MHC_BES 8
-#endif
-#ifndef MHC_BHS
-#define MHC_BHS true
-#endif
-#ifndef MHC_BB
-#define MHC_BB 1
-#endif
-#ifndef MHC_BBS
-#define MHC_BBS 1
-#endif
-#ifndef MHC_BT
-#define MHC_BT 2
-#endif
-#ifndef MHC_BTS
-#define MHC_BTS 1
-#endif
-#ifndef MHC_BTH
-#define MHC_BTH 512
-#endif
-#ifndef MHC_BTHS
-#define MHC_BTHS 512
-#endif
-constexpr int kNormBlock = 256;
-
-// One block per row, which it reads three times (the second and third come
-// from L1 or L2).
-template <class Elem, int kStreams>
-__global__ void __launch_bounds__(kNormBlock)
-norm_fwd_rows(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
-              float* __restrict__ rstd_out, float eps, int64_t N, int64_t C)
-{
-    __shared__ __align__(16) float buf[2][32];
-    const Group group{kNormBlock, static_cast<int>(threadIdx.x), 0};
-    group_sum_init<1>(group, buf[0]);
-    group_sum_init<1>(group, buf[1]);
-    for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-        const NormRow<Elem, kStreams> row(src, r);
-        float s[1] = {0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) s[0] += row.at(c);
-        group_sum(group, s, buf[0]);
-        const float mean = s[0] / static_cast<float>(C);
-        s[0] = 0.0f;
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
-            const float d = row.at(c) - mean;
-            s[0] = fmaf(d, d, s[0]);
-        }
-        group_sum(group, s, buf[1]);
-        const float rstd = rsqrtf(s[0] / static_cast<float>(C) + eps);
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
-            float v = (row.at(c) - mean) * rstd;
-            if (aff.w) v *= load_any(aff.w, c, aff.dtype);
-            if (aff.b) v += load_any(aff.b, c, aff.dtype);
-            y[r * C + c] = from_f32<Elem>(v);
-        }
-        if (threadIdx.x == 0) {
-            if (mean_out) mean_out[r] = mean;
-            if (rstd_out) rstd_out[r] = rstd;
-        }
-    }
-}
-
-template <class Elem, int kStreams>
-__global__ void __launch_bounds__(kNormBlock)
-norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kStreams> src,
-              const float* __restrict__ mean_in, const float* __restrict__ rstd_in, NormAffine aff,
-              Elem* __restrict__ dx, void* __restrict__ dh, int64_t N, int64_t C)
-{
-    __shared__ __align__(16) float buf[2 * 32];
-    __shared__ __align__(16) float buf_h[4 * 32];
-    const Group group{kNormBlock, static_cast<int>(threadIdx.x), 0};
-    group_sum_init<2>(group, buf);
-    group_sum_init<4>(group, buf_h);
-    for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-        const NormRow<Elem, kStreams> row(src, r);
-        const Elem* gr = g + r * g_stride;
-        const float mean = mean_in[r], rstd = rstd_in[r];
-        float s[2] = {0.0f, 0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
-            const float gw = to_f32(gr[c]) * (aff.w ? load_any(aff.w, c, aff.dtype) : 1.0f);
-            s[0] += gw;
-            s[1] = fmaf(gw, (row.at(c) - mean) * rstd, s[1]);
-        }
-        group_sum(group, s, buf);
-        const float m1 = s[0] / static_cast<float>(C), m2 = s[1] / static_cast<float>(C);
-        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
-            const float gw = to_f32(gr[c]) * (aff.w ? load_any(aff.w, c, aff.dtype) : 1.0f);
-            const float du = rstd * (gw - m1 - (row.at(c) - mean) * rstd * m2);
-            if constexpr (kStreams == 1) {
-                dx[r * C + c] = from_f32<Elem>(du);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kStreams; ++i) {
-                    a[i] = fmaf(du, to_f32(row.x[i * row.stream_stride + c]), a[i]);
-                    dx[(r * kStreams + i) * C + c] = from_f32<Elem>(row.h[i] * du);
-                }
-            }
-        }
-        if constexpr (kStreams > 1) {
-            group_sum(group, a, buf_h);
-            if (threadIdx.x == 0) {
-#pragma unroll
-                for (int i = 0; i < kStreams; ++i) store_any(dh, r * kStreams + i, src.h_dtype, a[i]);
-            }
-        }
-        __syncthreads();  // buf is written again
-    }
-}
-
-// Partial sums of dw and db over one chunk of rows: partials[chunk][0 or 1][C].
-constexpr int kParamRows = 8;  // rows a block works on at once, 32 columns wide
-
-template <class Elem, int kStreams>
-__global__ void __launch_bounds__(32 * kParamRows)
-norm_param_partials(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kStreams> src,
-                    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, float* __restrict__ partials,
-                    int64_t N, int64_t C, int64_t chunk_rows)
-{
-    __shared__ float part[2][kParamRows][32];
-    const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
-    const int64_t chunk = blockIdx.y, end = min(N, (chunk + 1) * chunk_rows);
-    for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32; c0 < C; c0 += static_cast<int64_t>(gridDim.x) * 32) {
-        const int64_t c = c0 + lane;
-        float dw = 0.0f, db = 0.0f;
-        if (c < C) {
-            for (int64_t r = chunk * chunk_rows + line; r < end; r += kParamRows) {
-                const NormRow<Elem, kStreams> row(src, r);
-                const float gv = to_f32(g[r * g_stride + c]);
-                dw = fmaf(gv, (row.at(c) - mean_in[r]) * rstd_in[r], dw);
-                db += gv;
-            }
-        }
-        part[0][line][lane] = dw;
-        part[1][line][lane] = db;
-        __syncthreads();
-        if (line < 2 && c < C) {
-            float v = part[line][0][lane];
-#pragma unroll
-            for (int k = 1; k < kParamRows; ++k) v += part[line][k][lane];
-            partials[(chunk * 2 + line) * C + c] = v;
-        }
-        __syncthreads();
-    }
-}
-
-// dw and db from `rows` rows of partial sums, 32 columns a block.
-constexpr int kFoldLines = 32;
-
-__global__ void __launch_bounds__(32 * kFoldLines)
-norm_param_fold(const float* __restrict__ partials, int64_t rows, void* __restrict__ dw, void* __restrict__ db,
-                int dtype, int64_t C)
-{
-    __shared__ float part[kFoldLines][33];
-    const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
-    void* out = blockIdx.y == 0 ? dw : db;
-    if (!out) return;
-    for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32; c0 < C; c0 += static_cast<int64_t>(gridDim.x) * 32) {
-        const int64_t c = c0 + lane;
-        float v = 0.0f;
-        if (c < C) {
-#pragma unroll 8
-            for (int64_t k = line; k < rows; k += kFoldLines) v += partials[(k * 2 + blockIdx.y) * C + c];
-        }
-        part[line][lane] = v;
-        __syncthreads();
-        // warp l folds column c0 + l
-        v = part[lane][line];
-#pragma unroll
-        for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-        if (lane == 0 && c0 + line < C) store_any(out, c0 + line, dtype, v);
-        __syncthreads();
-    }
-}
 
 constexpr int64_t kMaxRowGrid = int64_t{1} << 20;
 constexpr int64_t kParamChunks = 64;
@@ -214,11 +34,11 @@ constexpr int64_t kMaxPartials = 1024;
 
 static int64_t norm_workspace(int64_t N, int64_t C)
 {
-    return std::max<int64_t>(1, std::min(N, kMaxPartials)) * 2 * C * static_cast<int64_t>(sizeof(float));
+    return std::min(std::max<int64_t>(N, 16), kMaxPartials) * 2 * C * static_cast<int64_t>(sizeof(float));
 }
 
 // Whether rows move in 16-byte pieces: whole pieces, aligned, and the
-// parameters of a type that load_param reads in pieces.
+// parameters of a type that RowCols::param reads in pieces.
 template <class Elem, int kStreams>
 static bool norm_in_pieces(const NormSource<Elem, kStreams>& src, const NormAffine& aff, int64_t C)
 {
@@ -229,8 +49,16 @@ static bool norm_in_pieces(const NormSource<Elem, kStreams>& src, const NormAffi
            ((!aff.w && !aff.b) || aff.dtype == own || aff.dtype == MHC_DTYPE_F32);
 }
 
-// Elements of a row per thread and the most threads of a block, for rows of C
-// elements: more elements as the rows get wider.
+// Whether every row of x starts as far into 16 bytes as the same row of the
+// contiguous output does.
+template <class Elem>
+static bool lies_alike(const Elem* x, int64_t stride, const Elem* out, int64_t C)
+{
+    return ((reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
+           (((stride - C) * static_cast<int64_t>(sizeof(Elem))) & 15) == 0;
+}
+
+// The widest row that the held kernel takes, 512 threads with 32 elements each.
 constexpr int64_t kHeldMax = 32 * 512;
 
 template <class Elem, int kStreams, RowForm kForm, int kElems>
@@ -245,64 +73,101 @@ static void norm_forward_held(const NormSource<Elem, kStreams>& src, const NormA
 }
 
 // Calls `launch` with the form of the rows.
-template <class Launch>
-static cudaError_t by_form(bool pieces, bool whole, Launch launch)
+template <int kStreams, class Launch>
+static cudaError_t by_form(RowForm form, Launch launch)
 {
-    if (!pieces) return launch(std::integral_constant<RowForm, kLoose>{});
-    if (!whole) return launch(std::integral_constant<RowForm, kPieces>{});
-    return launch(std::integral_constant<RowForm, kWhole>{});
+    if constexpr (kStreams == 1) {
+        if (form == kSkewed) return launch(std::integral_constant<RowForm, kSkewed>{});
+    }
+    if (form == kWhole) return launch(std::integral_constant<RowForm, kWhole>{});
+    if (form == kPieces) return launch(std::integral_constant<RowForm, kPieces>{});
+    return launch(std::integral_constant<RowForm, kLoose>{});
 }
 
-// The ring kernels' shape for rows of C elements.
-struct RingPlan {
-    int threads, groups, stages, blocks_per_sm, smem;
-};
-
-// Elements of a row per thread, rows a turn and whether the parameters stay in
-// registers: rows of up to 8192 elements, and wider ones.
-template <int kStreams, bool kWide>
+// The ring kernels' shapes by width: elements of a row per thread, the most
+// threads of a group (their product is the widest row), rows a turn, and
+// whether the parameters stay in registers.  All are within 128 registers a
+// thread; a spill costs more than what the held values save.
+template <int kStreams, int kWidth>
 struct FwdShape {
-    static constexpr int kElems = kWide ? 32 : 16, kTurn = kStreams == 1 && !kWide ? 2 : 1;
+    static constexpr int kElems = kWidth ? 32 : 16, kTurn = kStreams == 1 && !kWidth ? 2 : 1;
+    static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
     static constexpr bool kHold = true;
+    static constexpr int kRows = kStreams * kTurn;  // of a stage
+    static constexpr int64_t kWidest = kElems * kMaxThreads;
 };
-template <class Elem, int kStreams, bool kWide>
+template <int kStreams, int kWidth>
 struct BwdShape {
-    static constexpr int kNarrow = kStreams == 1 ? MHC_BE : MHC_BES;
-    static constexpr int kElems = kWide ? 2 * kNarrow : kNarrow;
-    static constexpr bool kHold = kWide ? false : kStreams == 1 ? true : MHC_BHS;
-    static constexpr int kMaxThreads = 512;
+    static constexpr int kElems = kWidth == 2 ? 32 : kStreams == 1 || kWidth == 1 ? 16 : 8;
+    static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
+    static constexpr bool kHold = kWidth == 0 || (kStreams == 1 && kWidth == 1);
+    static constexpr int kRows = kStreams + 1;
+    static constexpr int64_t kWidest = kElems * kMaxThreads;
 };
-constexpr int64_t kNarrowMax = 16 * 512, kWideMax = 32 * 512;
-#ifndef MHC_MINST
-#define MHC_MINST 2
-#endif
-constexpr int kMinStages = MHC_MINST;
-constexpr int kRingSmem = MHC_SMEM * 1024;         // of an SM's 227 KB, for the ring
 
-static RingPlan ring_plan(int64_t C, int elem, bool vec, int rows, int per_thread, int threads_per_sm)
+// A ring kernel's launch.
+struct RingPlan {
+    RowForm form;
+    int width, elems, threads, groups, stages, blocks_per_sm, smem;
+
+    // Blocks for `turns` turns of the groups.
+    int64_t grid(int64_t turns, int elem) const
+    {
+        const int64_t blocks = std::min(ceil_div(turns, groups), static_cast<int64_t>(blocks_per_sm) * sm_count());
+        if (form != kSkewed) return blocks;
+        // the groups' turns go in steps of whole periods of 16 / elem rows
+        const int period = 16 / elem, unit = period / std::min(period, groups & -groups);
+        return std::max<int64_t>(unit, blocks / unit * unit);
+    }
+};
+
+// Of an SM's 227 KB, for the rings: more bytes under way are slower again.
+constexpr int ring_smem(int streams) { return (streams == 1 ? 100 : 150) * 1024; }
+
+// The shape (of kWidths) and launch for rows of C elements in `form`; stages 0: too wide.
+template <template <int, int> class Shape, int kStreams, int kWidths>
+static RingPlan ring_plan(int64_t C, int elem, RowForm form)
 {
-    RingPlan p;
-    p.threads = 32 * static_cast<int>(ceil_div(C, 32 * per_thread));
-    p.groups = p.threads == 32 ? 8 : std::max(1, 256 / p.threads);
-    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, vec, p.threads, per_thread) * p.groups;
-    p.blocks_per_sm = std::max(1, std::min(threads_per_sm / (p.threads * p.groups), kRingSmem / (kMinStages * stage)));
-    p.stages = std::min(kRingStages, std::max(1, kRingSmem / p.blocks_per_sm / stage));
+    RingPlan p{};
+    const int64_t span = C + (form == kSkewed ? 16 / elem - 1 : 0);  // columns from a piece's start
+    if (span > Shape<kStreams, kWidths - 1>::kWidest) return p;
+    int rows = Shape<kStreams, 0>::kRows;
+    p.elems = Shape<kStreams, 0>::kElems;
+    if (span > Shape<kStreams, 0>::kWidest) {
+        p.width = 1;
+        rows = Shape<kStreams, 1>::kRows;
+        p.elems = Shape<kStreams, 1>::kElems;
+    }
+    if (kWidths > 2 && span > Shape<kStreams, 1>::kWidest) {
+        p.width = 2;
+        rows = Shape<kStreams, kWidths - 1>::kRows;
+        p.elems = Shape<kStreams, kWidths - 1>::kElems;
+    }
+    const int64_t want = ceil_div(span, p.elems);
+    p.threads = 4;
+    while (p.threads < 32 && p.threads < want) p.threads *= 2;
+    if (want > 32) p.threads = 32 * static_cast<int>(ceil_div(want, 32));
+    p.form = form == kPieces && p.threads * p.elems == C ? kWhole : form;
+    p.groups = std::max(1, 256 / p.threads);
+    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, form == kLoose, p.threads, p.elems) * p.groups;
+    const int least = kStreams == 1 ? 1 : 2;  // stages
+    p.blocks_per_sm = std::max(1, std::min(kRingThreads / (p.threads * p.groups), ring_smem(kStreams) / (least * stage)));
+    p.stages = std::min(kRingStages, std::max(1, ring_smem(kStreams) / p.blocks_per_sm / stage));
     p.smem = std::max(p.stages * stage, p.groups > 1 ? static_cast<int>(8 * C) : 0);
-    if (stage > 225 * 1024) p.stages = 0;  // one row does not fit
+    if (stage > 208 * 1024) p.stages = 0;  // beside the static memory
     return p;
 }
 
-template <class Elem, int kStreams, RowForm kForm, bool kWide>
+template <class Elem, int kStreams, RowForm kForm, int kWidth>
 static cudaError_t norm_forward_ring(const RingPlan& p, const NormSource<Elem, kStreams>& src, const NormAffine& aff,
                                      Elem* y, float* mean, float* rstd, float eps, int64_t N, int64_t C,
                                      cudaStream_t stream)
 {
-    using S = FwdShape<kStreams, kWide>;
-    const auto kernel = norm_fwd_ring<Elem, kStreams, kForm, S::kElems, S::kTurn, S::kHold, 512>;
+    using S = FwdShape<kStreams, kWidth>;
+    const auto kernel = norm_fwd_ring<Elem, kStreams, kForm, S::kElems, S::kTurn, S::kHold, S::kMaxThreads>;
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
-    const int64_t grid = std::min<int64_t>(ceil_div(ceil_div(N, S::kTurn), p.groups), static_cast<int64_t>(p.blocks_per_sm) * sm_count());
-    kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
+    kernel<<<static_cast<unsigned>(p.grid(ceil_div(N, S::kTurn), sizeof(Elem))), dim3(p.threads, p.groups), p.smem, stream>>>(
         src, span_of(src.x, N, src.stride, kStreams, src.stream_stride, C), aff, y, mean, rstd, eps, N,
         static_cast<int>(C), p.stages);
     return cudaSuccess;
@@ -315,28 +180,27 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, co
 {
     const NormSource<Elem, kStreams> src{static_cast<const Elem*>(x), stride, stream_stride, h, h_dtype};
     Elem* yp = static_cast<Elem*>(y);
-    const bool pieces = norm_in_pieces(src, aff, C) && aligned16(y);
-    const bool wide = C > kNarrowMax;
-    const int elems = wide ? FwdShape<kStreams, true>::kElems : FwdShape<kStreams, false>::kElems;
-    const int turn = wide ? FwdShape<kStreams, true>::kTurn : FwdShape<kStreams, false>::kTurn;
-    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams * turn, elems, 512);
-    if (C <= kWideMax && plan.stages > 0 && N >= MHC_RING_N) {
-        const auto launch = [&](auto form) {
-            constexpr RowForm f = decltype(form)::value;
-            return wide ? norm_forward_ring<Elem, kStreams, f, true>(plan, src, aff, yp, mean, rstd, eps, N, C, stream)
-                        : norm_forward_ring<Elem, kStreams, f, false>(plan, src, aff, yp, mean, rstd, eps, N, C, stream);
-        };
-        const cudaError_t e = by_form(pieces, plan.threads * elems == C, launch);
+    const RowForm form = norm_in_pieces(src, aff, C) && aligned16(y)            ? kPieces
+                         : kStreams == 1 && lies_alike(src.x, stride, yp, C) ? kSkewed
+                                                                                : kLoose;
+    const RingPlan plan = ring_plan<FwdShape, kStreams, 2>(C, sizeof(Elem), form);
+    if (plan.stages > 0 && N >= MHC_RING_N) {
+        const cudaError_t e = by_form<kStreams>(plan.form, [&](auto f) {
+            constexpr RowForm form = decltype(f)::value;
+            return plan.width ? norm_forward_ring<Elem, kStreams, form, 1>(plan, src, aff, yp, mean, rstd, eps, N, C, stream)
+                              : norm_forward_ring<Elem, kStreams, form, 0>(plan, src, aff, yp, mean, rstd, eps, N, C, stream);
+        });
         if (e != cudaSuccess) return static_cast<int>(e);
-    } else if (C > kHeldMax)
+    } else if (C > kHeldMax) {
         norm_fwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
             src, aff, yp, mean, rstd, eps, N, C);
-    else if (C > 8 * 512)
-        pieces ? norm_forward_held<Elem, kStreams, kPieces, 32>(src, aff, yp, mean, rstd, eps, N, C, stream)
-               : norm_forward_held<Elem, kStreams, kLoose, 32>(src, aff, yp, mean, rstd, eps, N, C, stream);
-    else
-        pieces ? norm_forward_held<Elem, kStreams, kPieces, 8>(src, aff, yp, mean, rstd, eps, N, C, stream)
-               : norm_forward_held<Elem, kStreams, kLoose, 8>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    } else if (C > 8 * 512) {
+        form == kPieces ? norm_forward_held<Elem, kStreams, kPieces, 32>(src, aff, yp, mean, rstd, eps, N, C, stream)
+                        : norm_forward_held<Elem, kStreams, kLoose, 32>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    } else {
+        form == kPieces ? norm_forward_held<Elem, kStreams, kPieces, 8>(src, aff, yp, mean, rstd, eps, N, C, stream)
+                        : norm_forward_held<Elem, kStreams, kLoose, 8>(src, aff, yp, mean, rstd, eps, N, C, stream);
+    }
     return static_cast<int>(cudaGetLastError());
 }
 
@@ -363,13 +227,13 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, in
     }
 }
 
-template <class Elem, int kStreams, RowForm kForm, bool kWide>
+template <class Elem, int kStreams, RowForm kForm, int kWidth>
 static cudaError_t norm_backward_ring(const RingPlan& p, int64_t grid, const Elem* g, int64_t g_stride,
                                       const NormSource<Elem, kStreams>& src, const float* mean, const float* rstd,
                                       const NormAffine& aff, Elem* dx, void* dh, float* partials, int64_t N, int64_t C,
                                       cudaStream_t stream)
 {
-    using S = BwdShape<Elem, kStreams, kWide>;
+    using S = BwdShape<kStreams, kWidth>;
     const auto kernel = norm_bwd_ring<Elem, kStreams, kForm, S::kElems, S::kHold, S::kMaxThreads>;
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
@@ -380,6 +244,23 @@ static cudaError_t norm_backward_ring(const RingPlan& p, int64_t grid, const Ele
     return cudaSuccess;
 }
 
+// Launched so that its blocks may be set up while the kernel before it, which
+// makes the partial sums, still runs; they wait for its end.
+static cudaError_t fold_params(const float* partials, int64_t rows, void* dw, void* db, int dtype, int64_t C,
+                               cudaStream_t stream)
+{
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20)), 2);
+    config.blockDim = dim3(32 * kFoldLines);
+    config.stream = stream;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, norm_param_fold, partials, rows, dw, db, dtype, C);
+}
+
 template <class Elem, int kStreams>
 static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t stride, int64_t stream_stride,
                          const void* h, int h_dtype, const float* mean, const float* rstd, const NormAffine& aff,
@@ -388,41 +269,44 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
 {
     const NormSource<Elem, kStreams> src{static_cast<const Elem*>(x), stride, stream_stride, h, h_dtype};
     const Elem* gp = static_cast<const Elem*>(g);
-    const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
-    const bool pieces = norm_in_pieces(src, aff, C) && aligned16(g, g_stride, sizeof(Elem)) && aligned16(dx);
-    const bool wide = C > BwdShape<Elem, kStreams, false>::kElems * 512;
-    const int elems = wide ? BwdShape<Elem, kStreams, true>::kElems : BwdShape<Elem, kStreams, false>::kElems;
-    const RingPlan plan = ring_plan(C, sizeof(Elem), pieces, kStreams + 1, elems, kStreams == 1 ? MHC_BTH : MHC_BTHS);
-    if (N > 0 && plan.threads <= 512 && plan.stages > 0) {
-        const int64_t grid = std::min({ceil_div(N, plan.groups),
-                                       static_cast<int64_t>(plan.blocks_per_sm) * sm_count(), kMaxPartials});
-        float* part = dw || db ? partials : nullptr;
-        Elem* dxp = static_cast<Elem*>(dx);
-        const auto launch = [&](auto form) {
-            constexpr RowForm f = decltype(form)::value;
-            return wide ? norm_backward_ring<Elem, kStreams, f, true>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp,
-                                                                      dh, part, N, C, stream)
-                        : norm_backward_ring<Elem, kStreams, f, false>(plan, grid, gp, g_stride, src, mean, rstd, aff, dxp,
+    Elem* dxp = static_cast<Elem*>(dx);
+    float* part = dw || db ? partials : nullptr;
+    const RowForm form =
+        norm_in_pieces(src, aff, C) && aligned16(g, g_stride, sizeof(Elem)) && aligned16(dx)                  ? kPieces
+        : kStreams == 1 && lies_alike(src.x, stride, dxp, C) && lies_alike(gp, g_stride, dxp, C) ? kSkewed
+                                                                                                              : kLoose;
+    const RingPlan plan = ring_plan<BwdShape, kStreams, 3>(C, sizeof(Elem), form);
+    int64_t rows = 0;  // of partial sums
+    if (N > 0 && plan.stages > 0) {
+        rows = std::min(plan.grid(N, sizeof(Elem)), kMaxPartials);
+        const cudaError_t e = by_form<kStreams>(plan.form, [&](auto f) {
+            constexpr RowForm form = decltype(f)::value;
+            switch (plan.width) {
+                case 0:
+                    return norm_backward_ring<Elem, kStreams, form, 0>(plan, rows, gp, g_stride, src, mean, rstd, aff, dxp,
                                                                        dh, part, N, C, stream);
-        };
-        const cudaError_t e = by_form(pieces, plan.threads * elems == C, launch);
+                case 1:
+                    return norm_backward_ring<Elem, kStreams, form, 1>(plan, rows, gp, g_stride, src, mean, rstd, aff, dxp,
+                                                                       dh, part, N, C, stream);
+                default:
+                    return norm_backward_ring<Elem, kStreams, form, 2>(plan, rows, gp, g_stride, src, mean, rstd, aff, dxp,
+                                                                       dh, part, N, C, stream);
+            }
+        });
         if (e != cudaSuccess) return static_cast<int>(e);
-        if (part) norm_param_fold<<<dim3(cols, 2), 32 * kFoldLines, 0, stream>>>(partials, grid, dw, db, aff.dtype, C);
-        return static_cast<int>(cudaGetLastError());
-    }
-    if (N > 0)
+    } else if (N > 0) {
         norm_bwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
-            gp, g_stride, src, mean, rstd, aff, static_cast<Elem*>(dx), dh, N, C);
-    if (dw || db) {
-        int64_t chunks = 0;
-        if (N > 0) {
-            chunks = std::min(ceil_div(N, kParamRows), kParamChunks);
-            const int64_t chunk_rows = ceil_div(N, chunks);
-            norm_param_partials<Elem, kStreams>
-                <<<dim3(cols, static_cast<unsigned>(chunks)), 32 * kParamRows, 0, stream>>>(
-                    gp, g_stride, src, mean, rstd, partials, N, C, chunk_rows);
+            gp, g_stride, src, mean, rstd, aff, dxp, dh, N, C);
+        if (dw || db) {
+            rows = std::min(ceil_div(N, kParamRows), kParamChunks);
+            const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
+            norm_param_partials<Elem, kStreams><<<dim3(cols, static_cast<unsigned>(rows)), 32 * kParamRows, 0, stream>>>(
+                gp, g_stride, src, mean, rstd, partials, N, C, ceil_div(N, rows));
         }
-        norm_param_fold<<<dim3(cols, 2), 32 * kFoldLines, 0, stream>>>(partials, chunks, dw, db, aff.dtype, C);
+    }
+    if (dw || db) {
+        const cudaError_t e = fold_params(partials, rows, dw, db, aff.dtype, C, stream);
+        if (e != cudaSuccess) return static_cast<int>(e);
     }
     return static_cast<int>(cudaGetLastError());
 }

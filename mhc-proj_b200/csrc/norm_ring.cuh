@@ -1,17 +1,18 @@
 // Layer norm over rows that pass through a ring of stages in shared memory.
 //
-// A group of threads (one warp, or the whole block) takes row after row.  The
-// rows to come are copied into the ring by asynchronous copies of 16-byte
-// pieces that need no registers, so the bytes in flight do not depend on the
-// occupancy and the copies go on while the group reduces and stores a row.
+// A group of threads (some lanes of a warp, a warp, or several warps) takes row
+// after row.  The rows to come are copied into the ring by asynchronous copies of
+// 16-byte pieces that need no registers, so the bytes in flight do not depend
+// on the occupancy and the copies go on while the group reduces and stores a
+// row.
 //
-// Rows of aligned, whole pieces (kVec): every thread copies the pieces that it
-// reads itself, so that the wait for its own copies is all the
-// synchronisation a stage needs.  Any other rows: a stage keeps a row at the
-// offset within 16 bytes that it has in memory, the group copies all the
-// pieces that the row touches, and a barrier stands between that and the
-// reading of single elements, `threads` apart.  Pieces that reach beyond the
-// first or last byte of the tensor are copied element by element.
+// Rows in pieces (row_cols.cuh): every thread copies the pieces that it reads
+// itself, so that the wait for its own copies is all the synchronisation a
+// stage needs.  Loose rows: a stage keeps a row at the offset within 16 bytes
+// that it has in memory, the group copies all the pieces that the row touches,
+// and a barrier stands between that and the reading of single elements.  Pieces
+// that reach beyond the first or last byte of the tensor are copied element by
+// element.
 #pragma once
 
 #include "norm_source.cuh"
@@ -20,43 +21,50 @@
 
 namespace mhcp {
 
+constexpr int kRingThreads = 512;  // of an SM, in its rings' blocks
+
 // Bytes of one row's place in a stage.
-__host__ __device__ inline int ring_row_bytes(int C, int elem, bool vec, int threads, int per_thread)
+__host__ __device__ inline int ring_row_bytes(int C, int elem, bool loose, int threads, int per_thread)
 {
-    return vec ? threads * per_thread * elem : (C * elem + 15) / 16 * 16 + 16;
+    return loose ? (C * elem + 15) / 16 * 16 + 16 : threads * per_thread * elem;
 }
 
 // The ring of one group: kRows rows a stage, kElems elements of a row a thread.
 template <class Elem, int kRows, RowForm kForm, int kElems>
 struct RowRing {
-    static constexpr int kPiece = 16 / sizeof(Elem);
-    static constexpr int K = RowCols<Elem, kForm>::K;
-    static constexpr int P = kElems / K;
+    using Cols = RowCols<Elem, kForm>;
+    static constexpr int K = Cols::K, P = kElems / K;
 
     char* base;
-    int row_bytes, C, t, threads;
-    RowCols<Elem, kForm> cols;
+    int row_bytes;
+    const Cols& cols;
 
     __device__ __forceinline__ char* place(int stage, int row) const { return base + (stage * kRows + row) * row_bytes; }
+    __device__ __forceinline__ int piece(int p) const { return p * cols.threads + cols.t; }
 
     // amid: the tensor has 32 bytes on both sides of the row
     __device__ __forceinline__ void copy(int stage, int row, const Elem* from, const RowSpan& span, bool amid) const
     {
         char* to = place(stage, row);
         if constexpr (kForm != kLoose) {
+            const char* src = reinterpret_cast<const char*>(from - (kForm == kSkewed ? cols.skew : 0));
 #pragma unroll
             for (int p = 0; p < P; ++p) {
-                const int piece = p * threads + t;
-                if (cols.has(p)) copy_piece_async(to + piece * 16, from + piece * kPiece);
+                if (!cols.has(p)) continue;
+                if (kForm != kSkewed || amid || cols.all(p))
+                    copy_piece_async(to + piece(p) * 16, src + piece(p) * 16);
+                else
+                    copy_checked_piece(to + piece(p) * 16, src + piece(p) * 16, from, from + cols.C, span);
             }
         } else {
             const int skew = offset_in_piece(from);
-            const int pieces = (skew + C * static_cast<int>(sizeof(Elem)) + 15) >> 4;
+            const int pieces = (skew + cols.C * static_cast<int>(sizeof(Elem)) + 15) >> 4;
             const char* src = reinterpret_cast<const char*>(from) - skew;
             if (amid) {
-                for (int q = t; q < pieces; q += threads) copy_piece_async(to + 16 * q, src + 16 * q);
+                for (int q = cols.t; q < pieces; q += cols.threads) copy_piece_async(to + 16 * q, src + 16 * q);
             } else {
-                for (int q = t; q < pieces; q += threads) copy_checked_piece(to + 16 * q, src + 16 * q, from, from + C, span);
+                for (int q = cols.t; q < pieces; q += cols.threads)
+                    copy_checked_piece(to + 16 * q, src + 16 * q, from, from + cols.C, span);
             }
         }
     }
@@ -64,27 +72,32 @@ struct RowRing {
     // The 16 bytes of piece p of a row of a stage, of rows in pieces.
     __device__ __forceinline__ uint4 raw(int stage, int row, int p) const
     {
-        return cols.has(p) ? *reinterpret_cast<const uint4*>(place(stage, row) + (p * threads + t) * 16)
-                           : make_uint4(0, 0, 0, 0);
+        return cols.has(p) ? *reinterpret_cast<const uint4*>(place(stage, row) + piece(p) * 16) : make_uint4(0, 0, 0, 0);
     }
 
     // Piece p of a row of a stage; `from` is where the row came from.
     __device__ __forceinline__ void get(int stage, int row, int p, const Elem* from, float2 (&v)[K / 2]) const
     {
-        if constexpr (kForm != kLoose) {
-            cols.unpack(raw(stage, row, p), v);
-        } else {
+        if constexpr (kForm != kLoose)
+            cols.unpack(p, raw(stage, row, p), v);
+        else
             cols.load(p, reinterpret_cast<const Elem*>(place(stage, row) + offset_in_piece(from)), v);
-        }
     }
 };
 
-// Block: (threads of a row's group, groups); more groups than one only where a
-// group is a warp.  A group takes kTurn rows at a time, next to each other, so
-// that the weight and bias are read once for them and their sums share their
-// barriers; its turns are first + k * step.
+// How far into its first piece of 16 bytes a skewed row starts, in elements.
+template <class Elem, RowForm kForm>
+__device__ __forceinline__ int row_skew(const Elem* row)
+{
+    return kForm == kSkewed ? offset_in_piece(row) / static_cast<int>(sizeof(Elem)) : 0;
+}
+
+// Block: (threads of a row's group, groups).  A group takes kTurn rows at a time,
+// so that their sums share their barriers; its turns are first + k * step, where
+// step is a whole number of kTurn rows' period: rows `period` apart are skewed
+// alike.
 template <class Elem, int kStreams, RowForm kForm, int kElems, int kTurn, bool kHold, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kMaxThreads, kRingThreads / kMaxThreads)
 norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem* __restrict__ y,
               float* __restrict__ mean_out, float* __restrict__ rstd_out, float eps, int64_t N, int C, int stages)
 {
@@ -92,30 +105,26 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
     __shared__ __align__(16) float buf[kMaxGroups][2][kTurn * 32];
     using Ring = RowRing<Elem, kStreams * kTurn, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
-    const int threads = blockDim.x, t = threadIdx.x;
-    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm != kLoose, threads, kElems);
-    const RowCols<Elem, kForm> cols{C, t, threads};
-    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * kStreams * kTurn * row_bytes, row_bytes, C, t,
-                    threads, cols};
-    const Group group{threads, t, static_cast<int>(threadIdx.y)};
-    float(*sums)[kTurn * 32] = buf[threads > 32 ? threadIdx.y : 0];  // a warp's group needs none
-    if (threads > 32) {
-        group_sum_init<kTurn>(group, sums[0]);
-        group_sum_init<kTurn>(group, sums[1]);
-    }
-    const int64_t turns = (N + kTurn - 1) / kTurn;
+    const Group group;
+    constexpr int64_t period = kForm == kSkewed ? 16 / sizeof(Elem) : 1;
+    auto row_of = [&](int64_t turn, int q) { return turn / period * (period * kTurn) + turn % period + q * period; };
+    const int64_t turns = (N + period * kTurn - 1) / (period * kTurn) * period;
     const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-    // Row q of a turn; the last turn's rows beyond the batch are its last row once more.
-    auto row_of = [&](int64_t turn, int q) { return min(turn * kTurn + q, N - 1); };
+    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm == kLoose, group.threads, kElems);
+    const typename Ring::Cols cols(C, group.t, group.threads, row_skew<Elem, kForm>(src.x + row_of(first, 0) * src.stride));
+    const Ring ring{ring_memory + static_cast<size_t>(group.id) * stages * kStreams * kTurn * row_bytes, row_bytes, cols};
+    float(*sums)[kTurn * 32] = buf[group.one_warp() ? 0 : group.id];  // a warp's group needs none
+    group_sum_init<kTurn>(group, sums[0]);
+    group_sum_init<kTurn>(group, sums[1]);
     auto fill = [&](int stage, int64_t turn) {
-        if (turn < turns) {
 #pragma unroll
-            for (int q = 0; q < kTurn; ++q) {
+        for (int q = 0; q < kTurn; ++q) {
+            const int64_t r = row_of(turn, q);
+            if (r < N) {
 #pragma unroll
                 for (int i = 0; i < kStreams; ++i)
-                    ring.copy(stage, q * kStreams + i, src.x + row_of(turn, q) * src.stride + i * src.stream_stride, span,
-                              span.amid(row_of(turn, q), N));
+                    ring.copy(stage, q * kStreams + i, src.x + r * src.stride + i * src.stream_stride, span, span.amid(r, N));
             }
         }
         copies_commit();
@@ -136,7 +145,7 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
     NormRow<Elem, kStreams> next[kTurn];  // rows' weights are loaded one turn ahead
     auto look_ahead = [&](int64_t turn) {
 #pragma unroll
-        for (int q = 0; q < kTurn; ++q) next[q] = NormRow<Elem, kStreams>(src, row_of(min(turn, turns - 1), q));
+        for (int q = 0; q < kTurn; ++q) next[q] = NormRow<Elem, kStreams>(src, min(row_of(turn, q), N - 1));
     };
     look_ahead(first);
     for (int64_t turn = first; turn < turns; turn += step) {
@@ -182,7 +191,9 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
             for (int p = 0; p < P; ++p) {
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j) u[q][p][j] = add2(u[q][p][j], both(-mean[q]));
-                s2 = cols.squares(p, u[q][p], s2);
+                cols.clear_rest(p, u[q][p]);
+#pragma unroll
+                for (int j = 0; j < K / 2; ++j) s2 = fma2(u[q][p][j], u[q][p][j], s2);
             }
             s[q] = s2.x + s2.y;
         }
@@ -207,13 +218,13 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
                 float2 o[K / 2];
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j) o[j] = fma2(mul2(u[q][p][j], both(rstd[q])), w[j], b[j]);
-                if (turn * kTurn + q < N) cols.store(p, y + (turn * kTurn + q) * C, o);
+                if (row_of(turn, q) < N) cols.store(p, y + row_of(turn, q) * C, o);
             }
         }
-        if (t == 0) {
+        if (group.t == 0) {
 #pragma unroll
             for (int q = 0; q < kTurn; ++q) {
-                const int64_t r = turn * kTurn + q;
+                const int64_t r = row_of(turn, q);
                 if (r < N && mean_out) mean_out[r] = mean[q];
                 if (r < N && rstd_out) rstd_out[r] = rstd[q];
             }
@@ -251,7 +262,7 @@ __device__ __forceinline__ float warp_sum16(float (&v)[16])
 // m1 = sum(gw) / C, m2 = sum(gw xhat) / C.  A thread keeps its elements' gw and
 // xhat until then (of one stream: the 16-byte pieces of g and x as they are).
 template <class Elem, int kStreams, RowForm kForm, int kElems, bool kHold, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads)
+__global__ void __launch_bounds__(kMaxThreads, kRingThreads / kMaxThreads)
 norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, NormSource<Elem, kStreams> src,
               RowSpan span, const float* __restrict__ mean_in, const float* __restrict__ rstd_in, NormAffine aff,
               Elem* __restrict__ dx, void* __restrict__ dh, float* __restrict__ partials, int64_t N, int C, int stages)
@@ -262,19 +273,15 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
     constexpr int kRows = kStreams + 1;  // of a stage: the streams, then g
     using Ring = RowRing<Elem, kRows, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
-    const int threads = blockDim.x, t = threadIdx.x, warps = threads >> 5;
-    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm != kLoose, threads, kElems);
-    const RowCols<Elem, kForm> cols{C, t, threads};
-    const Ring ring{ring_memory + static_cast<size_t>(threadIdx.y) * stages * kRows * row_bytes, row_bytes, C, t, threads,
-                    cols};
-    const Group group{threads, t, static_cast<int>(threadIdx.y)};
-    float(*sums)[kSums * 32] = buf[threads > 32 ? threadIdx.y : 0];  // a warp's group needs none
-    if (threads > 32) {
-        group_sum_init<2>(group, sums[0]);
-        group_sum_init<2>(group, sums[1]);
-    }
+    const Group group;
     const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
+    const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm == kLoose, group.threads, kElems);
+    const typename Ring::Cols cols(C, group.t, group.threads, row_skew<Elem, kForm>(src.x + first * src.stride));
+    const Ring ring{ring_memory + static_cast<size_t>(group.id) * stages * kRows * row_bytes, row_bytes, cols};
+    float(*sums)[kSums * 32] = buf[group.one_warp() ? 0 : group.id];  // a warp's group needs none
+    group_sum_init<2>(group, sums[0]);
+    group_sum_init<2>(group, sums[1]);
     auto fill = [&](int stage, int64_t r) {
         if (r < N) {
 #pragma unroll
@@ -303,6 +310,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
         }
     };
     const float inv = 1.0f / static_cast<float>(C);
+    cudaTriggerProgrammaticLaunchCompletion();  // the fold may get ready
     int stage = 0, parity = 0;
     // a row's weights and statistics are loaded one row ahead
     int64_t ahead = min(first, N - 1);
@@ -331,8 +339,8 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             }
             auto piece = [&](int p, float2 (&gv)[K / 2], float2 (&u)[K / 2]) {
                 if constexpr (kForm != kLoose) {
-                    cols.unpack(kept[0][p], u);
-                    cols.unpack(kept[1][p], gv);
+                    cols.unpack(p, kept[0][p], u);
+                    cols.unpack(p, kept[1][p], gv);
                 } else {
                     ring.get(stage, 0, p, row.x, u);
                     ring.get(stage, 1, p, gr, gv);
@@ -413,38 +421,51 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 all[10 + i] = sh[i].x + sh[i].y;
             }
             all[14] = all[15] = 0.0f;
-            const float mine = warp_sum16(all);
-            float m1, m2, a, b, c;  // a, b, c: of stream t, in the group's first threads
-            if (threads == 32) {
+            float m1, m2, a = 0.0f, b = 0.0f, c = 0.0f;  // a, b, c: of stream t, in the group's first threads
+            if (group.threads < 32) {
+                group.lane_sum(all);
+                m1 = all[0];
+                m2 = all[1];
+#pragma unroll
+                for (int i = 0; i < kStreams; ++i) {
+                    if (group.t == i) {
+                        a = all[2 + i];
+                        b = all[6 + i];
+                        c = all[10 + i];
+                    }
+                }
+            } else if (group.threads == 32) {
+                const float mine = warp_sum16(all);
                 m1 = __shfl_sync(0xffffffffu, mine, 0);
                 m2 = __shfl_sync(0xffffffffu, mine, 1);
-                a = __shfl_sync(0xffffffffu, mine, 2 + (t & 3));
-                b = __shfl_sync(0xffffffffu, mine, 6 + (t & 3));
-                c = __shfl_sync(0xffffffffu, mine, 10 + (t & 3));
+                a = __shfl_sync(0xffffffffu, mine, 2 + (group.t & 3));
+                b = __shfl_sync(0xffffffffu, mine, 6 + (group.t & 3));
+                c = __shfl_sync(0xffffffffu, mine, 10 + (group.t & 3));
             } else {
                 // value k of warp w at [k][w]
                 float* part = sums[parity];
-                if ((t & 31) < 14) part[(t & 31) * 32 + (t >> 5)] = mine;
+                const float mine = warp_sum16(all);
+                if ((group.t & 31) < 14) part[(group.t & 31) * 32 + (group.t >> 5)] = mine;
                 group.sync();
-                m1 = m2 = a = b = c = 0.0f;
-                for (int k = 0; k < warps; k += 4) {  // parts of warps that the group does not have are zero
+                m1 = m2 = 0.0f;
+                for (int k = 0; k < group.warps(); k += 4) {  // parts of warps that the group does not have are zero
                     const float4 f = *reinterpret_cast<const float4*>(part + k);
                     const float4 h = *reinterpret_cast<const float4*>(part + 32 + k);
                     m1 += (f.x + f.y) + (f.z + f.w);
                     m2 += (h.x + h.y) + (h.z + h.w);
                 }
-                if (t < kStreams) {
-                    for (int k = 0; k < warps; ++k) {
-                        a += part[(2 + t) * 32 + k];
-                        b += part[(6 + t) * 32 + k];
-                        c += part[(10 + t) * 32 + k];
+                if (group.t < kStreams) {
+                    for (int k = 0; k < group.warps(); ++k) {
+                        a += part[(2 + group.t) * 32 + k];
+                        b += part[(6 + group.t) * 32 + k];
+                        c += part[(10 + group.t) * 32 + k];
                     }
                 }
             }
             if constexpr (kForm == kLoose) fill(stage, r + stages * step);  // all of the group have read the stage
             m1 *= inv;
             m2 *= inv;
-            if (t < kStreams) store_any(dh, r * kStreams + t, src.h_dtype, rstd * (a - m1 * b - m2 * c));
+            if (group.t < kStreams) store_any(dh, r * kStreams + group.t, src.h_dtype, rstd * (a - m1 * b - m2 * c));
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
@@ -474,7 +495,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             for (int p = 0; p < P; ++p) {
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
-                    if (!cols.has(p, j)) continue;
+                    if (!cols.in(p, j)) continue;
                     const int c = cols.col(p, j);
                     float &a = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x, &b = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
                     if (k > 0) {
@@ -492,7 +513,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
     for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            if (!cols.has(p, j)) continue;
+            if (!cols.in(p, j)) continue;
             out[cols.col(p, j)] = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x;
             out[C + cols.col(p, j)] = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
         }
@@ -510,14 +531,12 @@ norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__
     using Cols = RowCols<Elem, kForm>;
     constexpr int K = Cols::K, P = kElems / K;
     __shared__ __align__(16) float buf[2][32];
-    const Group group{static_cast<int>(blockDim.x), static_cast<int>(threadIdx.x), 0};
-    if (blockDim.x > 32) {
-        group_sum_init<1>(group, buf[0]);
-        group_sum_init<1>(group, buf[1]);
-    }
+    const Group group;  // of whole warps; more than one in the block only where it is one warp
+    group_sum_init<1>(group, buf[0]);
+    group_sum_init<1>(group, buf[1]);
     const int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y;
     if (r >= N) return;
-    const Cols cols{C, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    const Cols cols(C, group.t, group.threads, 0);
     const NormRow<Elem, kStreams> row(src, r);
     float2 u[P][K / 2];
     float2 s2 = both(0.0f);
@@ -555,7 +574,9 @@ norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__
     for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int j = 0; j < K / 2; ++j) u[p][j] = add2(u[p][j], both(-mean));
-        s2 = cols.squares(p, u[p], s2);
+        cols.clear_rest(p, u[p]);
+#pragma unroll
+        for (int j = 0; j < K / 2; ++j) s2 = fma2(u[p][j], u[p][j], s2);
     }
     s[0] = s2.x + s2.y;
     group_sum(group, s, buf[1]);

@@ -1,10 +1,13 @@
-// A thread's columns of a row that a group of threads holds: pieces p of K
-// columns, in pairs.
-//   VecCols     16-byte pieces, the group's next to each other.  For rows whose
-//               starts are 16-byte aligned and whose width is whole pieces (kFull:
-//               all the pieces that the group's threads take).
-//   LooseCols   single columns, the group's threads next to each other; any
-//               width and alignment, each column in the row or not.
+// A thread's columns of a row that a group of threads holds: P pieces of K
+// columns, in pairs.  The forms of rows that the kernels are built for:
+//   kLoose    any rows: single columns, the group's threads next to each other
+//   kSkewed   16-byte pieces as they lie in memory, where a row's first and
+//             last piece may be shared with its neighbours.  For rows that lie
+//             the same way in all of their tensors; a group takes rows that
+//             lie `skew` elements into their first piece, all of them
+//   kPieces   rows of whole, aligned pieces
+//   kWhole    the same, and exactly as many as the group's threads take, so
+//             that nothing is asked per piece
 // What is not in the row reads as zero (or what the caller names) and is not
 // written.
 #pragma once
@@ -13,38 +16,66 @@
 
 namespace mhcp {
 
-template <class Elem, bool kFull>
-struct VecCols {
-    static constexpr bool kVec = true;
+enum RowForm { kLoose, kSkewed, kPieces, kWhole };
+
+template <class Elem, RowForm kForm>
+struct RowCols {  // in pieces
     static constexpr int K = 16 / sizeof(Elem);
-    int C, t, threads;
+    int C, t, threads, skew;
 
-    __device__ __forceinline__ int col(int p, int j) const { return (p * threads + t) * K + j; }
-    __device__ __forceinline__ bool has(int p, int = 0) const { return kFull || col(p, 0) < C; }
+    __device__ __forceinline__ RowCols(int width, int thread, int of, int skewed)
+        : C(width), t(thread), threads(of), skew(kForm == kSkewed ? skewed : 0)
+    {
+    }
+    __device__ __forceinline__ int col(int p, int j) const
+    {
+        return (p * threads + t) * K + j - (kForm == kSkewed ? skew : 0);
+    }
+    // Whether something of piece p is in the row, and whether all of it is.
+    __device__ __forceinline__ bool has(int p) const { return kForm == kWhole || col(p, 0) < C; }
+    __device__ __forceinline__ bool all(int p) const
+    {
+        return kForm != kSkewed || (col(p, 0) >= 0 && col(p, 0) + K <= C);
+    }
+    __device__ __forceinline__ bool in(int p, int j) const
+    {
+        if constexpr (kForm != kSkewed) return has(p);
+        return static_cast<unsigned>(col(p, j)) < static_cast<unsigned>(C);
+    }
 
-    static __device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[K / 2])
+    __device__ __forceinline__ void unpack(int p, const uint4& q, float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) v[i] = pair_of<Elem>(q, i);
+        if constexpr (kForm == kSkewed) clear_rest(p, v);
     }
-
     __device__ __forceinline__ void load(int p, const Elem* __restrict__ row, float2 (&v)[K / 2]) const
     {
-        unpack(has(p) ? __ldg(reinterpret_cast<const uint4*>(row + col(p, 0))) : make_uint4(0, 0, 0, 0), v);
+        unpack(p, has(p) ? __ldg(reinterpret_cast<const uint4*>(row + col(p, 0))) : make_uint4(0, 0, 0, 0), v);
     }
-
     __device__ __forceinline__ void store(int p, Elem* __restrict__ row, const float2 (&v)[K / 2]) const
     {
-        const uint4 q = piece_of<Elem>(v);
-        if (has(p)) *reinterpret_cast<uint4*>(row + col(p, 0)) = q;
+        if (!has(p)) return;
+        if (all(p)) {
+            *reinterpret_cast<uint4*>(row + col(p, 0)) = piece_of<Elem>(v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (in(p, j)) row[col(p, j)] = from_f32<Elem>(j & 1 ? v[j / 2].y : v[j / 2].x);
+        }
     }
-
-    // A norm's weight or bias: of the rows' own type or fp32, aligned (the launcher's rule).
+    // A norm's weight or bias: in pieces of the rows' own type or fp32, aligned (the launcher's rule).
     __device__ __forceinline__ void param(int p, const void* a, int dtype, float none, float2 (&v)[K / 2]) const
     {
         if (!a) {
 #pragma unroll
             for (int i = 0; i < K / 2; ++i) v[i] = both(none);
+        } else if constexpr (kForm == kSkewed) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                const float f = in(p, j) ? load_any(a, col(p, j), dtype) : none;
+                (j & 1 ? v[j / 2].y : v[j / 2].x) = f;
+            }
         } else if (sizeof(Elem) == 4 || dtype != MHC_DTYPE_F32) {
             load(p, static_cast<const Elem*>(a), v);
         } else {
@@ -57,83 +88,66 @@ struct VecCols {
             }
         }
     }
-
-    // Pairs of v that are in the row, the others zero.
     __device__ __forceinline__ void clear_rest(int p, float2 (&v)[K / 2]) const
     {
+        if constexpr (kForm == kWhole) return;
+        if (has(p) && all(p)) return;
 #pragma unroll
-        for (int i = 0; i < K / 2; ++i) v[i] = has(p) ? v[i] : both(0.0f);
-    }
-    // Sum of squares of the pairs that are in the row.
-    __device__ __forceinline__ float2 squares(int p, const float2 (&v)[K / 2], float2 sum) const
-    {
-        float2 d = both(0.0f);
-#pragma unroll
-        for (int i = 0; i < K / 2; ++i) d = fma2(v[i], v[i], d);
-        return has(p) ? add2(sum, d) : sum;
+        for (int i = 0; i < K / 2; ++i) {
+            if (!in(p, 2 * i)) v[i].x = 0.0f;
+            if (!in(p, 2 * i + 1)) v[i].y = 0.0f;
+        }
     }
 };
 
 template <class Elem>
-struct LooseCols {
-    static constexpr bool kVec = false;
+struct RowCols<Elem, kLoose> {
     static constexpr int K = 8;
     int C, t, threads;
+    int steps, mine;  // columns of the first and of this thread
 
+    __device__ __forceinline__ RowCols(int width, int thread, int of, int)
+        : C(width), t(thread), threads(of), steps((width + of - 1) / of), mine((width - thread + of - 1) / of)
+    {
+    }
     __device__ __forceinline__ int col(int p, int j) const { return (p * K + j) * threads + t; }
-    __device__ __forceinline__ bool has(int p, int j) const { return col(p, j) < C; }
+    __device__ __forceinline__ bool in(int p, int j) const { return p * K + j < mine; }
 
     __device__ __forceinline__ void load(int p, const Elem* row, float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            v[i].x = has(p, 2 * i) ? to_f32(row[col(p, 2 * i)]) : 0.0f;
-            v[i].y = has(p, 2 * i + 1) ? to_f32(row[col(p, 2 * i + 1)]) : 0.0f;
+            v[i] = both(0.0f);
+            if (p * K + 2 * i >= steps) continue;
+            if (in(p, 2 * i)) v[i].x = to_f32(row[col(p, 2 * i)]);
+            if (in(p, 2 * i + 1)) v[i].y = to_f32(row[col(p, 2 * i + 1)]);
         }
     }
-
     __device__ __forceinline__ void store(int p, Elem* __restrict__ row, const float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            if (has(p, 2 * i)) row[col(p, 2 * i)] = from_f32<Elem>(v[i].x);
-            if (has(p, 2 * i + 1)) row[col(p, 2 * i + 1)] = from_f32<Elem>(v[i].y);
+            if (p * K + 2 * i >= steps) continue;
+            if (in(p, 2 * i)) row[col(p, 2 * i)] = from_f32<Elem>(v[i].x);
+            if (in(p, 2 * i + 1)) row[col(p, 2 * i + 1)] = from_f32<Elem>(v[i].y);
         }
     }
-
     __device__ __forceinline__ void param(int p, const void* a, int dtype, float none, float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            v[i].x = a && has(p, 2 * i) ? load_any(a, col(p, 2 * i), dtype) : none;
-            v[i].y = a && has(p, 2 * i + 1) ? load_any(a, col(p, 2 * i + 1), dtype) : none;
+            v[i].x = a && in(p, 2 * i) ? load_any(a, col(p, 2 * i), dtype) : none;
+            v[i].y = a && in(p, 2 * i + 1) ? load_any(a, col(p, 2 * i + 1), dtype) : none;
         }
     }
-
     __device__ __forceinline__ void clear_rest(int p, float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            if (!has(p, 2 * i)) v[i].x = 0.0f;
-            if (!has(p, 2 * i + 1)) v[i].y = 0.0f;
+            if (!in(p, 2 * i)) v[i].x = 0.0f;
+            if (!in(p, 2 * i + 1)) v[i].y = 0.0f;
         }
-    }
-    __device__ __forceinline__ float2 squares(int p, const float2 (&v)[K / 2], float2 sum) const
-    {
-#pragma unroll
-        for (int i = 0; i < K / 2; ++i) {
-            const float2 d = make_float2(has(p, 2 * i) ? v[i].x : 0.0f, has(p, 2 * i + 1) ? v[i].y : 0.0f);
-            sum = fma2(d, d, sum);
-        }
-        return sum;
     }
 };
-
-// The three forms that the kernels are built for.  kWhole: pieces, and exactly
-// as many as the group's threads take, so that nothing is asked per piece.
-enum RowForm { kLoose, kPieces, kWhole };
-
-template <class Elem, RowForm kForm>
-using RowCols = typename std::conditional<kForm == kLoose, LooseCols<Elem>, VecCols<Elem, kForm == kWhole>>::type;
 
 }  // namespace mhcp

@@ -89,19 +89,39 @@ __device__ __forceinline__ uint4 piece_of(const float2 (&v)[kPairs])
 // Widths are ints in the kernels.
 constexpr int64_t kMaxWidth = int64_t{1} << 30;
 
-// The threads that work on one row: a warp, or several warps of a block, which
-// may hold other groups (each has a barrier of its own).
+// The threads that work on one row: 4, 8, 16 or 32 lanes of a warp, or several
+// whole warps; a block may hold more than one such group, block (threads,
+// groups), and each has a barrier of its own.
 struct Group {
     int threads, t, id;
+    unsigned lanes;  // of the warp, the group's
+
+    __device__ __forceinline__ Group()
+        : threads(blockDim.x), t(threadIdx.x), id(threadIdx.y),
+          lanes(blockDim.x >= 32 ? 0xffffffffu
+                                 : ((1u << blockDim.x) - 1) << (threadIdx.x + threadIdx.y * blockDim.x & 31 & ~(blockDim.x - 1)))
+    {
+    }
+    __device__ __forceinline__ bool one_warp() const { return threads <= 32; }
+    __device__ __forceinline__ int warps() const { return threads >> 5; }
 
     __device__ __forceinline__ void sync() const
     {
-        if (threads == 32)
-            __syncwarp();
+        if (threads <= 32)
+            __syncwarp(lanes);
         else if (blockDim.y == 1)
             __syncthreads();
         else
             asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+    }
+    // Sums over the group's lanes of a warp.
+    template <int K>
+    __device__ __forceinline__ void lane_sum(float (&v)[K]) const
+    {
+        for (int m = min(threads, 32) >> 1; m > 0; m >>= 1) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(lanes, v[k], m);
+        }
     }
 };
 
@@ -115,7 +135,7 @@ template <int K>
 __device__ __forceinline__ void group_sum_init(const Group& g, float* buf)
 {
     // parts of warps that the group does not have: added as zeros
-    if (g.t >= g.threads >> 5 && g.t < 32) {
+    if (!g.one_warp() && g.t >= g.warps() && g.t < 32) {
 #pragma unroll
         for (int k = 0; k < K; ++k) buf[k * 32 + g.t] = 0.0f;
     }
@@ -124,12 +144,15 @@ __device__ __forceinline__ void group_sum_init(const Group& g, float* buf)
 template <int K>
 __device__ __forceinline__ void group_sum(const Group& g, float (&v)[K], float* buf)
 {
+    if (g.one_warp()) {
+        g.lane_sum(v);
+        return;
+    }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) {
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
     }
-    if (g.threads == 32) return;
     if ((g.t & 31) == 0) {
 #pragma unroll
         for (int k = 0; k < K; ++k) buf[k * 32 + (g.t >> 5)] = v[k];
@@ -138,7 +161,7 @@ __device__ __forceinline__ void group_sum(const Group& g, float (&v)[K], float* 
     float4 f[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) f[k] = *reinterpret_cast<const float4*>(buf + k * 32);
-    for (int w = 4; w < g.threads >> 5; w += 4) {
+    for (int w = 4; w < g.warps(); w += 4) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const float4 o = *reinterpret_cast<const float4*>(buf + k * 32 + w);
