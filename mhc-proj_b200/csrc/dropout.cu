@@ -10,7 +10,6 @@
 namespace mhcp {
 
 constexpr int kDropBlock = 256;
-constexpr int kDropGroups = 4;  // groups a thread takes
 
 // A group of eight elements, one counter's draws, from and to 16-byte aligned memory.
 template <class Elem>
@@ -28,34 +27,47 @@ struct DropGroup {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p)[i] = q[i];
     }
-    __device__ __forceinline__ void drop(uint32_t keep, float scale)
+    // The eight draws are the halves of w, low one first; an element is kept
+    // when its draw, in the upper half of a word, is above `under`.
+    __device__ __forceinline__ void drop(const uint4& draws, uint32_t under, float scale)
     {
-        Elem* e = reinterpret_cast<Elem*>(q);
+        const uint32_t w[4] = {draws.x, draws.y, draws.z, draws.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f32<Elem>((keep >> i & 1u) ? to_f32(e[i]) * scale : 0.0f);
+        for (int i = 0; i < kPieces; ++i) {
+            float2 v[16 / sizeof(Elem) / 2];
+#pragma unroll
+            for (int j = 0; j < 16 / static_cast<int>(sizeof(Elem)) / 2; ++j) {
+                const uint32_t d = w[i * (16 / sizeof(Elem) / 2) + j];
+                v[j] = mul2(pair_of<Elem>(q[i], j), both(scale));
+                if (d << 16 <= under) v[j].x = 0.0f;
+                if (d <= under) v[j].y = 0.0f;
+            }
+            q[i] = piece_of<Elem>(v);
+        }
     }
 };
 
-template <class Elem, bool kVec>
+// kGroups: groups a thread takes.
+template <class Elem, bool kVec, int kGroups>
 __global__ void __launch_bounds__(kDropBlock)
 dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
 {
     const uint2 key = dropout_key(d);
-    const int64_t q0 = blockIdx.x * static_cast<int64_t>(kDropBlock * kDropGroups) + threadIdx.x;
+    const int64_t q0 = blockIdx.x * static_cast<int64_t>(kDropBlock * kGroups) + threadIdx.x;
     const int64_t whole = count / 8;
-    if (kVec && q0 + (kDropGroups - 1) * kDropBlock < whole) {
-        DropGroup<Elem> g[kDropGroups];
+    if (kVec && q0 + (kGroups - 1) * kDropBlock < whole) {
+        DropGroup<Elem> g[kGroups];
 #pragma unroll
-        for (int k = 0; k < kDropGroups; ++k) g[k].load(x + 8 * (q0 + k * kDropBlock));
+        for (int k = 0; k < kGroups; ++k) g[k].load(x + 8 * (q0 + k * kDropBlock));
 #pragma unroll
-        for (int k = 0; k < kDropGroups; ++k) {
+        for (int k = 0; k < kGroups; ++k) {
             const int64_t q = q0 + k * kDropBlock;
-            g[k].drop(d.limit ? keep_bits(q, d.offset, key, d.limit) : 0xffu, d.scale);
+            if (d.limit) g[k].drop(draws_of(q, d.offset, key), (d.limit << 16) - 1, d.scale);
             g[k].store(y + 8 * q);
         }
         return;
     }
-    for (int k = 0; k < kDropGroups; ++k) {
+    for (int k = 0; k < kGroups; ++k) {
         const int64_t q = q0 + k * kDropBlock, e = 8 * q;
         if (e >= count) return;
         const uint32_t keep = d.limit ? keep_bits(q, d.offset, key, d.limit) : 0xffu;
@@ -65,18 +77,26 @@ dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
     }
 }
 
-template <class Elem>
-static int dropout_launch(const void* x, void* y, int64_t count, const Dropout& d, cudaStream_t stream)
+template <class Elem, bool kVec, int kGroups>
+static int dropout_launch(const Elem* x, Elem* y, int64_t count, const Dropout& d, cudaStream_t stream)
 {
-    const int64_t blocks = ceil_div(count, 8 * kDropBlock * kDropGroups);
+    const int64_t blocks = ceil_div(count, 8 * kDropBlock * kGroups);
     if (blocks > 0x7fffffff) return MHC_ERR_INVALID_VALUE;
+    dropout_kernel<Elem, kVec, kGroups><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(x, y, count, d);
+    return static_cast<int>(cudaGetLastError());
+}
+
+// Four groups a thread where the batch fills the GPU several times over (bf16,
+// 65536 x 4096: 177 us against 202 with one), one where it does not (fp32, 4099 x
+// 1111: 6.3 us against 7.7) and for fp32, whose groups are two pieces.
+template <class Elem>
+static int dropout_typed(const void* x, void* y, int64_t count, const Dropout& d, cudaStream_t stream)
+{
     const Elem* xe = static_cast<const Elem*>(x);
     Elem* ye = static_cast<Elem*>(y);
-    if (aligned16(x) && aligned16(y))
-        dropout_kernel<Elem, true><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(xe, ye, count, d);
-    else
-        dropout_kernel<Elem, false><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(xe, ye, count, d);
-    return static_cast<int>(cudaGetLastError());
+    if (!aligned16(x) || !aligned16(y)) return dropout_launch<Elem, false, 1>(xe, ye, count, d, stream);
+    if (sizeof(Elem) == 4 || count < (int64_t{1} << 23)) return dropout_launch<Elem, true, 1>(xe, ye, count, d, stream);
+    return dropout_launch<Elem, true, 4>(xe, ye, count, d, stream);
 }
 
 }  // namespace mhcp
@@ -91,8 +111,8 @@ extern "C" int mhc_dropout(const void* d_x, void* d_y, int dtype, int64_t count,
     if (count == 0) return MHC_OK;
     const Dropout d = make_dropout(p, seed, d_seed, offset);
     switch (dtype) {
-        case MHC_DTYPE_BF16: return dropout_launch<__nv_bfloat16>(d_x, d_y, count, d, stream);
-        case MHC_DTYPE_F16: return dropout_launch<__half>(d_x, d_y, count, d, stream);
-        default: return dropout_launch<float>(d_x, d_y, count, d, stream);
+        case MHC_DTYPE_BF16: return dropout_typed<__nv_bfloat16>(d_x, d_y, count, d, stream);
+        case MHC_DTYPE_F16: return dropout_typed<__half>(d_x, d_y, count, d, stream);
+        default: return dropout_typed<float>(d_x, d_y, count, d, stream);
     }
 }

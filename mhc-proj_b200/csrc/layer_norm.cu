@@ -144,7 +144,7 @@ static RingPlan ring_plan(int64_t C, int elem, RowForm form)
         p.elems = Shape<kStreams, kWidths - 1>::kElems;
     }
     const int64_t want = ceil_div(span, p.elems);
-    p.threads = 4;
+    p.threads = form == kLoose ? 32 : 4;
     while (p.threads < 32 && p.threads < want) p.threads *= 2;
     if (want > 32) p.threads = 32 * static_cast<int>(ceil_div(want, 32));
     p.form = form == kPieces && p.threads * p.elems == C ? kWhole : form;

@@ -32,7 +32,7 @@ __host__ __device__ inline int ring_row_bytes(int C, int elem, bool loose, int t
 // The ring of one group: kRows rows a stage, kElems elements of a row a thread.
 template <class Elem, int kRows, RowForm kForm, int kElems>
 struct RowRing {
-    using Cols = RowCols<Elem, kForm>;
+    using Cols = RowCols<Elem, kForm, kElems>;
     static constexpr int K = Cols::K, P = kElems / K;
 
     char* base;
@@ -69,6 +69,23 @@ struct RowRing {
         }
     }
 
+    // What a skewed row's first and last pieces have of its neighbours, to
+    // zero: once per row, by the threads that read them.
+    __device__ __forceinline__ void trim(int stage, int row) const
+    {
+        if constexpr (kForm == kSkewed) {
+            if (!cols.edge) return;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                if (!cols.has(p) || cols.all(p)) continue;
+                Elem* e = reinterpret_cast<Elem*>(place(stage, row) + piece(p) * 16);
+#pragma unroll
+                for (int j = 0; j < K; ++j)
+                    if (!cols.in(p, j)) e[j] = from_f32<Elem>(0.0f);
+            }
+        }
+    }
+
     // The 16 bytes of piece p of a row of a stage, of rows in pieces.
     __device__ __forceinline__ uint4 raw(int stage, int row, int p) const
     {
@@ -79,7 +96,7 @@ struct RowRing {
     __device__ __forceinline__ void get(int stage, int row, int p, const Elem* from, float2 (&v)[K / 2]) const
     {
         if constexpr (kForm != kLoose)
-            cols.unpack(p, raw(stage, row, p), v);
+            cols.unpack(raw(stage, row, p), v);
         else
             cols.load(p, reinterpret_cast<const Elem*>(place(stage, row) + offset_in_piece(from)), v);
     }
@@ -159,6 +176,7 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
         float s[kTurn];
 #pragma unroll
         for (int q = 0; q < kTurn; ++q) {
+            ring.trim(stage, q * kStreams);
             float2 s2 = both(0.0f);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -330,6 +348,8 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             // Rows in pieces are kept as they are; other rows are read from the stage twice.
             uint4 kept[kForm != kLoose ? 2 : 1][P];
             if constexpr (kForm != kLoose) {
+                ring.trim(stage, 0);
+                ring.trim(stage, 1);
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
                     kept[0][p] = ring.raw(stage, 0, p);
@@ -339,8 +359,8 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             }
             auto piece = [&](int p, float2 (&gv)[K / 2], float2 (&u)[K / 2]) {
                 if constexpr (kForm != kLoose) {
-                    cols.unpack(p, kept[0][p], u);
-                    cols.unpack(p, kept[1][p], gv);
+                    cols.unpack(kept[0][p], u);
+                    cols.unpack(kept[1][p], gv);
                 } else {
                     ring.get(stage, 0, p, row.x, u);
                     ring.get(stage, 1, p, gr, gv);
@@ -528,7 +548,7 @@ __global__ void __launch_bounds__(kMaxThreads)
 norm_fwd_held(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__ y, float* __restrict__ mean_out,
               float* __restrict__ rstd_out, float eps, int64_t N, int C)
 {
-    using Cols = RowCols<Elem, kForm>;
+    using Cols = RowCols<Elem, kForm, kElems>;
     constexpr int K = Cols::K, P = kElems / K;
     __shared__ __align__(16) float buf[2][32];
     const Group group;  // of whole warps; more than one in the block only where it is one warp

@@ -57,18 +57,25 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k)
     return c;
 }
 
-// Bit i: element 8 * group + i is kept.
+// The 128 bits that hold the draws of elements 8 * group ...
+__device__ __forceinline__ uint4 draws_of(uint64_t group, uint64_t offset, uint2 key)
+{
+    return philox4x32_10(make_uint4(static_cast<uint32_t>(group), static_cast<uint32_t>(group >> 32),
+                                    static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
+                         key);
+}
+
+// Bit i: element 8 * group + i is kept.  limit is not 0.
 __device__ __forceinline__ uint32_t keep_bits(uint64_t group, uint64_t offset, uint2 key, uint32_t limit)
 {
-    const uint4 v = philox4x32_10(make_uint4(static_cast<uint32_t>(group), static_cast<uint32_t>(group >> 32),
-                                             static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
-                                  key);
+    const uint4 v = draws_of(group, offset, key);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t under = (limit << 16) - 1;  // a draw in a word's upper half is kept above it
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        bits |= (w[i] & 0xffffu) >= limit ? 1u << (2 * i) : 0u;
-        bits |= (w[i] >> 16) >= limit ? 2u << (2 * i) : 0u;
+        bits |= w[i] << 16 > under ? 1u << (2 * i) : 0u;
+        bits |= w[i] > under ? 2u << (2 * i) : 0u;
     }
     return bits;
 }

@@ -1,6 +1,6 @@
-// A thread's columns of a row that a group of threads holds: P pieces of K
+// A thread's kElems columns of a row that a group of threads holds: pieces of K
 // columns, in pairs.  The forms of rows that the kernels are built for:
-//   kLoose    any rows: single columns, the group's threads next to each other
+//   kLoose    any rows: single columns, a warp's threads next to each other
 //   kSkewed   16-byte pieces as they lie in memory, where a row's first and
 //             last piece may be shared with its neighbours.  For rows that lie
 //             the same way in all of their tensors; a group takes rows that
@@ -18,14 +18,19 @@ namespace mhcp {
 
 enum RowForm { kLoose, kSkewed, kPieces, kWhole };
 
-template <class Elem, RowForm kForm>
+template <class Elem, RowForm kForm, int kElems>
 struct RowCols {  // in pieces
     static constexpr int K = 16 / sizeof(Elem);
     int C, t, threads, skew;
+    bool edge;  // one of this thread's pieces is only partly in the row
 
     __device__ __forceinline__ RowCols(int width, int thread, int of, int skewed)
-        : C(width), t(thread), threads(of), skew(kForm == kSkewed ? skewed : 0)
+        : C(width), t(thread), threads(of), skew(kForm == kSkewed ? skewed : 0), edge(false)
     {
+        if constexpr (kForm == kSkewed) {
+            const int end = (C + skew) % K;  // of the last piece
+            edge = (t == 0 && skew) || (end && t == (C + skew) / K % threads);
+        }
     }
     __device__ __forceinline__ int col(int p, int j) const
     {
@@ -43,20 +48,19 @@ struct RowCols {  // in pieces
         return static_cast<unsigned>(col(p, j)) < static_cast<unsigned>(C);
     }
 
-    __device__ __forceinline__ void unpack(int p, const uint4& q, float2 (&v)[K / 2]) const
+    static __device__ __forceinline__ void unpack(const uint4& q, float2 (&v)[K / 2])
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) v[i] = pair_of<Elem>(q, i);
-        if constexpr (kForm == kSkewed) clear_rest(p, v);
     }
     __device__ __forceinline__ void load(int p, const Elem* __restrict__ row, float2 (&v)[K / 2]) const
     {
-        unpack(p, has(p) ? __ldg(reinterpret_cast<const uint4*>(row + col(p, 0))) : make_uint4(0, 0, 0, 0), v);
+        unpack(has(p) ? __ldg(reinterpret_cast<const uint4*>(row + col(p, 0))) : make_uint4(0, 0, 0, 0), v);
     }
     __device__ __forceinline__ void store(int p, Elem* __restrict__ row, const float2 (&v)[K / 2]) const
     {
         if (!has(p)) return;
-        if (all(p)) {
+        if (!edge || all(p)) {
             *reinterpret_cast<uint4*>(row + col(p, 0)) = piece_of<Elem>(v);
         } else {
 #pragma unroll
@@ -91,7 +95,7 @@ struct RowCols {  // in pieces
     __device__ __forceinline__ void clear_rest(int p, float2 (&v)[K / 2]) const
     {
         if constexpr (kForm == kWhole) return;
-        if (has(p) && all(p)) return;
+        if (has(p) && (!edge || all(p))) return;
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
             if (!in(p, 2 * i)) v[i].x = 0.0f;
@@ -100,36 +104,34 @@ struct RowCols {  // in pieces
     }
 };
 
-template <class Elem>
-struct RowCols<Elem, kLoose> {
+template <class Elem, int kElems>
+struct RowCols<Elem, kLoose, kElems> {
     static constexpr int K = 8;
     int C, t, threads;
-    int steps, mine;  // columns of the first and of this thread
+    int first, rest;  // this thread's first column, and the row's columns from there
 
     __device__ __forceinline__ RowCols(int width, int thread, int of, int)
-        : C(width), t(thread), threads(of), steps((width + of - 1) / of), mine((width - thread + of - 1) / of)
+        : C(width), t(thread), threads(of), first((thread >> 5) * (32 * kElems) + (thread & 31)), rest(width - first)
     {
     }
-    __device__ __forceinline__ int col(int p, int j) const { return (p * K + j) * threads + t; }
-    __device__ __forceinline__ bool in(int p, int j) const { return p * K + j < mine; }
+    // a warp's columns are next to each other, a thread's 32 apart
+    __device__ __forceinline__ int col(int p, int j) const { return first + (p * K + j) * 32; }
+    __device__ __forceinline__ bool in(int p, int j) const { return (p * K + j) * 32 < rest; }
 
     __device__ __forceinline__ void load(int p, const Elem* row, float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            v[i] = both(0.0f);
-            if (p * K + 2 * i >= steps) continue;
-            if (in(p, 2 * i)) v[i].x = to_f32(row[col(p, 2 * i)]);
-            if (in(p, 2 * i + 1)) v[i].y = to_f32(row[col(p, 2 * i + 1)]);
+            v[i].x = in(p, 2 * i) ? to_f32((row + first)[(p * K + 2 * i) * 32]) : 0.0f;
+            v[i].y = in(p, 2 * i + 1) ? to_f32((row + first)[(p * K + 2 * i + 1) * 32]) : 0.0f;
         }
     }
     __device__ __forceinline__ void store(int p, Elem* __restrict__ row, const float2 (&v)[K / 2]) const
     {
 #pragma unroll
         for (int i = 0; i < K / 2; ++i) {
-            if (p * K + 2 * i >= steps) continue;
-            if (in(p, 2 * i)) row[col(p, 2 * i)] = from_f32<Elem>(v[i].x);
-            if (in(p, 2 * i + 1)) row[col(p, 2 * i + 1)] = from_f32<Elem>(v[i].y);
+            if (in(p, 2 * i)) (row + first)[(p * K + 2 * i) * 32] = from_f32<Elem>(v[i].x);
+            if (in(p, 2 * i + 1)) (row + first)[(p * K + 2 * i + 1) * 32] = from_f32<Elem>(v[i].y);
         }
     }
     __device__ __forceinline__ void param(int p, const void* a, int dtype, float none, float2 (&v)[K / 2]) const
