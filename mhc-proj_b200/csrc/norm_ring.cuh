@@ -75,13 +75,17 @@ struct RowRing {
     {
         if constexpr (kForm == kSkewed) {
             if (!cols.edge) return;
+            if (cols.t == 0) {
+                Elem* e = reinterpret_cast<Elem*>(place(stage, row));
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                if (!cols.has(p) || cols.all(p)) continue;
-                Elem* e = reinterpret_cast<Elem*>(place(stage, row) + piece(p) * 16);
+                for (int j = 0; j < K - 1; ++j)
+                    if (j < cols.skew) e[j] = from_f32<Elem>(0.0f);
+            }
+            if (cols.last()) {
+                Elem* e = reinterpret_cast<Elem*>(place(stage, row) + (cols.C + cols.skew) / K * 16);
 #pragma unroll
-                for (int j = 0; j < K; ++j)
-                    if (!cols.in(p, j)) e[j] = from_f32<Elem>(0.0f);
+                for (int j = 1; j < K; ++j)
+                    if (j >= cols.end) e[j] = from_f32<Elem>(0.0f);
             }
         }
     }
@@ -113,8 +117,8 @@ __device__ __forceinline__ int row_skew(const Elem* row)
 // so that their sums share their barriers; its turns are first + k * step, where
 // step is a whole number of kTurn rows' period: rows `period` apart are skewed
 // alike.
-template <class Elem, int kStreams, RowForm kForm, int kElems, int kTurn, bool kHold, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads, kRingThreads / kMaxThreads)
+template <class Elem, int kStreams, RowForm kForm, int kElems, int kTurn, bool kHold>
+__global__ void __launch_bounds__(kRingThreads, 1)
 norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem* __restrict__ y,
               float* __restrict__ mean_out, float* __restrict__ rstd_out, float eps, int64_t N, int C, int stages)
 {
@@ -279,8 +283,8 @@ __device__ __forceinline__ float warp_sum16(float (&v)[16])
 //   dh[i] = sum(du X[i]) = rstd (sum(gw X[i]) - m1 sum(X[i]) - m2 sum(xhat X[i])),
 // m1 = sum(gw) / C, m2 = sum(gw xhat) / C.  A thread keeps its elements' gw and
 // xhat until then (of one stream: the 16-byte pieces of g and x as they are).
-template <class Elem, int kStreams, RowForm kForm, int kElems, bool kHold, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads, kRingThreads / kMaxThreads)
+template <class Elem, int kStreams, RowForm kForm, int kElems, bool kHold>
+__global__ void __launch_bounds__(kRingThreads, 1)
 norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, NormSource<Elem, kStreams> src,
               RowSpan span, const float* __restrict__ mean_in, const float* __restrict__ rstd_in, NormAffine aff,
               Elem* __restrict__ dx, void* __restrict__ dh, float* __restrict__ partials, int64_t N, int C, int stages)

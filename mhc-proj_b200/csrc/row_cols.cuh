@@ -18,20 +18,47 @@ namespace mhcp {
 
 enum RowForm { kLoose, kSkewed, kPieces, kWhole };
 
+// An array of Param at single columns of a thread.
+template <class Param, class Cols, int kPairs>
+__device__ __forceinline__ void load_columns(const Cols& cols, int p, const void* a, float none, float2 (&v)[kPairs])
+{
+    const Param* q = static_cast<const Param*>(a);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        v[i].x = cols.in(p, 2 * i) ? to_f32(q[cols.col(p, 2 * i)]) : none;
+        v[i].y = cols.in(p, 2 * i + 1) ? to_f32(q[cols.col(p, 2 * i + 1)]) : none;
+    }
+}
+
+template <class Cols, int kPairs>
+__device__ __forceinline__ void load_columns(const Cols& cols, int p, const void* a, int dtype, float none,
+                                             float2 (&v)[kPairs])
+{
+    if (dtype == MHC_DTYPE_F32)
+        load_columns<float>(cols, p, a, none, v);
+    else if (dtype == MHC_DTYPE_BF16)
+        load_columns<__nv_bfloat16>(cols, p, a, none, v);
+    else
+        load_columns<__half>(cols, p, a, none, v);
+}
+
 template <class Elem, RowForm kForm, int kElems>
 struct RowCols {  // in pieces
     static constexpr int K = 16 / sizeof(Elem);
     int C, t, threads, skew;
-    bool edge;  // one of this thread's pieces is only partly in the row
+    int end;     // elements of the last piece, where they are not all of it
+    bool edge;   // one of this thread's pieces is only partly in the row
 
     __device__ __forceinline__ RowCols(int width, int thread, int of, int skewed)
-        : C(width), t(thread), threads(of), skew(kForm == kSkewed ? skewed : 0), edge(false)
+        : C(width), t(thread), threads(of), skew(kForm == kSkewed ? skewed : 0), end(0), edge(false)
     {
         if constexpr (kForm == kSkewed) {
-            const int end = (C + skew) % K;  // of the last piece
-            edge = (t == 0 && skew) || (end && t == (C + skew) / K % threads);
+            end = (C + skew) % K;
+            edge = (t == 0 && skew) || last();
         }
     }
+    // Whether the last piece is this thread's and not whole.
+    __device__ __forceinline__ bool last() const { return end && t == (C + skew) / K % threads; }
     __device__ __forceinline__ int col(int p, int j) const
     {
         return (p * threads + t) * K + j - (kForm == kSkewed ? skew : 0);
@@ -75,11 +102,7 @@ struct RowCols {  // in pieces
 #pragma unroll
             for (int i = 0; i < K / 2; ++i) v[i] = both(none);
         } else if constexpr (kForm == kSkewed) {
-#pragma unroll
-            for (int j = 0; j < K; ++j) {
-                const float f = in(p, j) ? load_any(a, col(p, j), dtype) : none;
-                (j & 1 ? v[j / 2].y : v[j / 2].x) = f;
-            }
+            load_columns(*this, p, a, dtype, none, v);
         } else if (sizeof(Elem) == 4 || dtype != MHC_DTYPE_F32) {
             load(p, static_cast<const Elem*>(a), v);
         } else {
@@ -136,10 +159,11 @@ struct RowCols<Elem, kLoose, kElems> {
     }
     __device__ __forceinline__ void param(int p, const void* a, int dtype, float none, float2 (&v)[K / 2]) const
     {
+        if (a) {
+            load_columns(*this, p, a, dtype, none, v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < K / 2; ++i) {
-            v[i].x = a && in(p, 2 * i) ? load_any(a, col(p, 2 * i), dtype) : none;
-            v[i].y = a && in(p, 2 * i + 1) ? load_any(a, col(p, 2 * i + 1), dtype) : none;
+            for (int i = 0; i < K / 2; ++i) v[i] = both(none);
         }
     }
     __device__ __forceinline__ void clear_rest(int p, float2 (&v)[K / 2]) const

@@ -396,6 +396,35 @@ def test_stream_mix_empty_batch():
     assert g["d_T"].shape == (0, 4, 4) and g["d_y"].shape == (0, 8)
 
 
+# ---- neighbours ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,C", [(9, 1001), (700, 33), (700, 1001), (700, 1025), (700, 72), (5, 4097)])
+def test_non_finite_rows_stay_alone(N, C, dtype, bad):
+    """Rows of odd widths share 16-byte pieces with their neighbours: every
+    second row of all inputs is non-finite, the others keep their results."""
+    g = gen(45)
+    X, y, G4, G = streams(N, C, g, dtype), normal(g, N, C).to(dtype), normal(g, N, 4, C).to(dtype), rows(N, C, g, dtype)
+    h, T = torch.sigmoid(normal(g, N, 4)), mixing(N, g)
+
+    def call():
+        a, s = f.layer_norm(y), f.stream_norm_n4(X, h)
+        m = f.stream_mix_n4(X, T, y, h, 0.1, 3)
+        outs = [a, s, m, f.layer_norm_backward(G, y, a["mean"], a["rstd"]),
+                f.stream_norm_n4_backward(G, X, h, s["mean"], s["rstd"]),
+                f.stream_mix_n4_backward(G4, X, T, y, h, 0.1, 3)]
+        return {f"{i}{k}": v for i, o in enumerate(outs) for k, v in o.items()}
+
+    want = call()
+    for t in (X, y, G4, G):
+        t[1::2] = bad
+    got = call()
+    for k in want:
+        assert same_bits(got[k][::2], want[k][::2]), k
+        assert not bool(torch.isfinite(got[k][1::2]).all()), k
+
+
 # ---- all of them ------------------------------------------------------------------------
 
 def all_calls(dtype, N, C, seed, drop_seed=7):
