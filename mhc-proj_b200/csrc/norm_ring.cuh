@@ -370,6 +370,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                     ring.get(stage, 1, p, gr, gv);
                 }
             };
+            const float shift = -mean * rstd;  // xhat = u rstd + shift
             float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -378,7 +379,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 weight(p, w);
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j) {  // g is zero beyond the row
-                    const float2 xhat = mul2(add2(u[j], both(-mean)), both(rstd));
+                    const float2 xhat = fma2(u[j], both(rstd), both(shift));
                     const float2 gw = mul2(gv[j], w[j]);
                     s0 = add2(s0, gw);
                     s1 = fma2(gw, xhat, s1);
@@ -388,8 +389,9 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             }
             float s[2] = {s0.x + s0.y, s1.x + s1.y};
             group_sum(group, s, sums[parity]);
-            // du = rstd (gw - m1 - (u - mean) rstd m2)
-            const float m1 = s[0] * inv, m2 = -s[1] * inv * rstd;
+            // du = rstd (gw - m1 - xhat m2) = g (w rstd) + (u slope + level)
+            const float m1 = s[0] * inv, m2 = s[1] * inv;
+            const float slope = -rstd * rstd * m2, level = -rstd * (m1 + shift * m2);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 float2 du[K / 2], u[K / 2], w[K / 2];
@@ -397,7 +399,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 weight(p, w);
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j)
-                    du[j] = mul2(both(rstd), fma2(add2(u[j], both(-mean)), both(m2), fma2(du[j], w[j], both(-m1))));
+                    du[j] = fma2(du[j], mul2(w[j], both(rstd)), fma2(u[j], both(slope), both(level)));
                 cols.store(p, dx + r * C, du);
             }
             if constexpr (kForm == kLoose) {
@@ -405,6 +407,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 fill(stage, r + stages * step);
             }
         } else {
+            const float shift = -mean * rstd;  // xhat = u rstd + shift
             float2 gw[P][K / 2], xhat[P][K / 2];
             float2 s0 = both(0.0f), s1 = both(0.0f), sx[kStreams], sg[kStreams], sh[kStreams];
 #pragma unroll
@@ -421,7 +424,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                     float2 u = mul2(v[0][j], both(row.h[0]));
 #pragma unroll
                     for (int i = 1; i < kStreams; ++i) u = fma2(v[i][j], both(row.h[i]), u);
-                    const float2 x = mul2(add2(u, both(-mean)), both(rstd)), y = mul2(gv[j], w[j]);
+                    const float2 x = fma2(u, both(rstd), both(shift)), y = mul2(gv[j], w[j]);
                     s0 = add2(s0, y);
                     s1 = fma2(y, x, s1);
                     dw[p][j] = fma2(gv[j], x, dw[p][j]);
@@ -494,7 +497,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             for (int p = 0; p < P; ++p) {
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j)
-                    gw[p][j] = mul2(both(rstd), fma2(xhat[p][j], both(-m2), add2(gw[p][j], both(-m1))));
+                    gw[p][j] = fma2(gw[p][j], both(rstd), fma2(xhat[p][j], both(-m2 * rstd), both(-m1 * rstd)));
 #pragma unroll
                 for (int i = 0; i < kStreams; ++i) {
                     float2 v[K / 2];
