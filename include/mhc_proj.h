@@ -1,11 +1,13 @@
 /*
  * mhc_proj -- batched n=4 Birkhoff projection on B200 (sm_100a).
  *
- * C ABI of libmhcproj.so.  Every entry point takes device pointers to N
- * contiguous row-major 4x4 fp32 matrices (64 bytes each), launches on
- * `stream` and returns without synchronising.  Pointers that are 16-byte
- * aligned take the 128-bit load/store path; any other alignment is accepted
- * and served by a scalar path.  Inputs and outputs must not overlap.
+ * C ABI of libmhcproj.so.  Every entry point takes device pointers -- to N
+ * contiguous row-major 4x4 fp32 matrices (64 bytes each) where its declaration
+ * names nothing else -- launches on `stream` and returns without synchronising.
+ * Pointers that are 16-byte aligned take the 128-bit load/store path; any other
+ * alignment (to the element) is accepted and served by other paths.  Inputs and
+ * outputs must not overlap.  Calls from several host threads do not disturb one
+ * another.
  *
  * Return value: MHC_OK (0), a negative MHC_ERR_* code for a rejected argument
  * (nothing is launched), or a positive cudaError_t from the launch.
@@ -35,7 +37,8 @@ extern "C" {
 enum {
     MHC_OK = 0,
     MHC_ERR_INVALID_VALUE = -1, /* N < 0, a null pointer with N > 0, a negative stride, an unknown dtype, or
-                                   (residual path) a width < 1, eps < 0, p outside [0, 1] or too small a workspace */
+                                   (residual path) N > 2^31 - 1, a width < 1 or > 2^30, eps < 0, p outside [0, 1] or
+                                   too small a workspace */
     MHC_ERR_ITERS = -2,         /* iteration count outside the supported range */
     MHC_ERR_CAPTURE = -3        /* a first call in a CUDA context that must look up a device
                                    address was made during stream capture */
@@ -318,9 +321,11 @@ MHC_API int mhc_sinkhorn_knopp_n4_hres_backward(const float* d_G, const float* d
  *
  * Rows of C elements of one storage type (`dtype`), fp32 arithmetic and sums,
  * one rounding per output.  A row's elements are contiguous; strides are in
- * elements and non-negative; outputs are contiguous.  C >= 1 is any width and
- * any alignment is accepted (rows whose starts are 16-byte aligned and whose
- * width is a multiple of 16 bytes move in 16-byte pieces).  No reference
+ * elements and non-negative; outputs are contiguous.  1 <= C <= 2^30 is any
+ * width, 0 <= N < 2^31, and any alignment is accepted (rows whose starts are
+ * 16-byte aligned and whose width is a multiple of 16 bytes move in 16-byte
+ * pieces).  Tensors must lie in memory as a whole: the bytes between the rows of
+ * a strided one may be read (their values are not used).  No reference
  * counterparts. */
 
 /* y = (x - mean) * rstd * w + b per row, rstd = 1 / sqrt(var + eps) with the
@@ -338,7 +343,8 @@ MHC_API int mhc_layer_norm_backward_workspace(int64_t N, int64_t C, int64_t* byt
 /* Gradients of mhc_layer_norm given g = dL/dy and the forward's mean and rstd:
  * dx (N x C, dtype), and dw and db (C elements of w_dtype), each of which may
  * be null.  dw and db are overwritten (zeros for N = 0).  Their sums over the
- * rows are deterministic: the same N, C and GPU model give the same bits.
+ * rows are deterministic: the same inputs at the same strides and alignment
+ * give the same bits on the same GPU model.
  * The call owns the workspace until it completes on `stream`; it may be null
  * when neither dw nor db is asked for. */
 MHC_API int mhc_layer_norm_backward(const void* d_g, int64_t g_stride, const void* d_x, int64_t x_stride, int dtype,

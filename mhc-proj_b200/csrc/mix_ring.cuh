@@ -2,6 +2,11 @@
 // shared memory: each warp copies the chunks it will take next, without
 // registers, while it works on one; no barrier of a block stands anywhere.  A
 // lane works on a piece of K consecutive columns, 16 bytes of each row.
+// Bound by HBM.  65536 tokens of 2048 bf16: forward 375 us, 6.4 TB/s (a block per
+// token with direct loads 643, a warp per token 458, this ring without packed
+// arithmetic 420); backward 595 us, 6.3 TB/s (a block per token 3220 with a sum
+// over it for each of the 20 coefficients' gradients, a warp per token with
+// direct loads 633), 631 under a load of seconds, when the clock falls.
 //   kVec   rows of aligned, whole pieces: `lanes` lanes (a power of two) share a
 //          token, 32 / lanes tokens a warp, and each lane copies what it reads.
 //   else   any rows of any width: the warp copies the aligned pieces that a
@@ -17,6 +22,8 @@
 namespace mhcp {
 
 constexpr int kMixRingBlock = 128;
+// Blocks of an SM and their stages: as many bytes under way as keep HBM busy; more
+// (forward 4 stages: 429 us for 375) meet one another in the memory system.
 constexpr int kMixFwdStages = 2, kMixBwdStages = 2, kMixFwdBlocks = 4;
 
 template <class Elem, bool kVec>

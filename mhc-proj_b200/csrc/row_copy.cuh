@@ -81,14 +81,19 @@ inline int sm_count()
     return sms;
 }
 
+// The dynamic shared memory of a launch at most; the kernels' static memory (16
+// KB at most) fits beside it.
+constexpr int kMostSmem = 200 * 1024;
+
 // A launch may need more dynamic shared memory than a kernel has by default
-// (48 KB, less what is static); the attribute belongs to the context, so it is
-// set for each such launch.
+// (48 KB, less what is static).  The limit belongs to the kernel in the context
+// and not to the launch, so every launch sets the same one: two host threads
+// with rows of two widths do not undo each other's.
 template <class Kernel>
 inline cudaError_t allow_smem(Kernel kernel, int bytes)
 {
     return bytes <= 32 * 1024 ? cudaSuccess
-                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
 }
 
 }  // namespace mhcp

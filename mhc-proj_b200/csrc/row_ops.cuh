@@ -86,8 +86,10 @@ __device__ __forceinline__ uint4 piece_of(const float2 (&v)[kPairs])
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Widths are ints in the kernels.
-constexpr int64_t kMaxWidth = int64_t{1} << 30;
+// Widths are ints in the kernels, rows a dimension of a grid.
+constexpr int64_t kMaxWidth = int64_t{1} << 30, kMaxRows = (int64_t{1} << 31) - 1;
+
+inline bool rows_ok(int64_t N, int64_t C) { return N >= 0 && N <= kMaxRows && C >= 1 && C <= kMaxWidth; }
 
 // The threads that work on one row: 4, 8, 16 or 32 lanes of a warp, or several
 // whole warps; a block may hold more than one such group, block (threads,

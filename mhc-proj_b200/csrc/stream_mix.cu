@@ -280,8 +280,9 @@ static int mix_backward_ring(const Elem* g, int64_t g_stride, int64_t g_stream_s
     const cudaError_t e = allow_smem(mix_bwd_ring<Elem, kVec, kWide>, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int lanes = kVec ? mix_threads(C / Chunk::K, 1, 32) : 32;
-    // Two blocks an SM, or three where a token is over before the next one's
-    // coefficients have come, or single elements take more instructions.
+    // Two blocks an SM (65536 tokens of 2048, bf16: 595 us, with three 675), or
+    // three where a token is over before the next one's coefficients have come,
+    // or single elements take more instructions.
     const int blocks = kVec && Chunk::count(static_cast<int>(C), lanes) > 2 ? 2 : 3;
     const int64_t grid = std::min<int64_t>(ceil_div(ceil_div(N, 32 / lanes), warps), blocks * sm_count());
     mix_bwd_ring<Elem, kVec, kWide><<<static_cast<unsigned>(grid), kMixRingBlock, smem, stream>>>(
@@ -300,7 +301,9 @@ static int mix_backward(const void* g, int64_t g_stride, int64_t g_stream_stride
     const bool pieces = mix_in_pieces(in, C) && aligned_streams(g, g_stride, g_stream_stride, sizeof(Elem)) &&
                         aligned16(dx) && aligned16(dy);
     const bool narrow = !pieces && C < kMixNarrow;
-    // A warp per token once there are four tokens for every SM, else a block.
+    // A warp per token once there are four tokens for every SM, else a block
+    // (bf16, 4096 wide: 300 tokens 14.0 us a warp each, 11.3 a block each; 1000
+    // tokens 23.6 and 30.4).
     if (N >= 4 * sm_count() && !narrow)
         return pieces ? mix_backward_ring<Elem, true, kWide>(gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, C, stream)
                       : mix_backward_ring<Elem, false, kWide>(gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, C, stream);
@@ -321,8 +324,8 @@ static bool mix_args_ok(const void* X, int64_t token_stride, int64_t stream_stri
                         int dtype, const void* T, int T_dtype, const void* h, int h_dtype, double p, int64_t N,
                         int64_t C)
 {
-    return N >= 0 && N < (int64_t{1} << 31) && C >= 1 && C <= kMaxWidth && token_stride >= 0 && stream_stride >= 0 &&
-           y_stride >= 0 && known_dtype(dtype) && known_dtype(T_dtype) && known_dtype(h_dtype) && p >= 0.0 && p <= 1.0 &&
+    return rows_ok(N, C) && token_stride >= 0 && stream_stride >= 0 && y_stride >= 0 && known_dtype(dtype) &&
+           known_dtype(T_dtype) && known_dtype(h_dtype) && p >= 0.0 && p <= 1.0 &&
            (N == 0 || (X && y && T && h));
 }
 

@@ -1,6 +1,7 @@
 """The residual path's kernels against the operators in 64 bits
 (residual_reference.py, where the bounds are derived)."""
 import gc
+import threading
 
 import pytest
 import torch
@@ -467,6 +468,50 @@ def test_other_streams_and_two_at_once():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(same_bits(x, y) for x, y in zip(a, b))
+
+
+def test_host_threads_at_once():
+    """Two host threads in one kernel with rows of two widths, which need
+    different amounts of shared memory: neither call fails or changes the
+    other's results."""
+    g = gen(58)
+    xs = [normal(g, 1200, C).bfloat16() for C in (1000, 2000)]
+    Xs = [normal(g, 700, 4, C).bfloat16() for C in (520, 1000)]
+    hs = [torch.rand(700, 4, device="cuda", generator=g) for _ in Xs]
+
+    def work(i):
+        o = f.layer_norm(xs[i])
+        u = capi_layer_norm(xs[i])
+        d = f.stream_norm_n4(Xs[i], hs[i])
+        return o["y"], u, d["y"]
+
+    def capi_layer_norm(x):
+        y = torch.empty_like(x)
+        capi.layer_norm(x.data_ptr(), x.stride(0), capi.MHC_DTYPE_BF16, 0, 0, capi.MHC_DTYPE_F32, y.data_ptr(), 0, 0,
+                        1e-5, *x.shape, torch.cuda.current_stream().cuda_stream)
+        return y
+
+    want = [work(i) for i in range(2)]
+    bad = []
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(400):
+                    got = work(i)
+                    if k % 100 == 99 and not all(same_bits(a, b) for a, b in zip(got, want[i])):
+                        bad.append((i, k))
+        except Exception as e:
+            bad.append((i, e))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad
 
 
 def test_captured_and_replayed_with_another_seed():
