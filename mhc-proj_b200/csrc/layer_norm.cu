@@ -94,6 +94,7 @@ struct FwdShape {
     static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
     static constexpr bool kHold = true;
     static constexpr int kRows = kStreams * kTurn;  // of a stage
+    static constexpr bool kSums = false;            // of the parameters' gradients, in shared memory at the end
     static constexpr int64_t kWidest = kElems * kMaxThreads;
 };
 template <int kStreams, int kWidth>
@@ -102,6 +103,7 @@ struct BwdShape {
     static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
     static constexpr bool kHold = kWidth == 0 || (kStreams == 1 && kWidth == 1);
     static constexpr int kRows = kStreams + 1;
+    static constexpr bool kSums = true;
     static constexpr int64_t kWidest = kElems * kMaxThreads;
 };
 
@@ -150,12 +152,18 @@ static RingPlan ring_plan(int64_t C, int elem, RowForm form)
     while (p.threads < 32 && p.threads < want) p.threads *= 2;
     if (want > 32) p.threads = 32 * static_cast<int>(ceil_div(want, 32));
     p.form = form == kPieces && p.threads * p.elems == C ? kWhole : form;
-    p.groups = std::max(1, 256 / p.threads);
-    const int stage = rows * ring_row_bytes(static_cast<int>(C), elem, form == kLoose, p.threads, p.elems) * p.groups;
+    const int row_stage = rows * ring_row_bytes(static_cast<int>(C), elem, form == kLoose, p.threads, p.elems);
     const int least = kStreams == 1 ? 1 : 2;  // stages
+    // The sums' rows of two blocks an SM cost skewed rows more than their waits for
+    // one another in one block (backward, bf16, 20003 x 1025: 57 us in blocks of 512
+    // threads, 61 of 256; whole pieces, 65536 x 4096: 269 and 263).
+    p.groups = std::max(1, (Shape<kStreams, 0>::kSums && form == kSkewed ? 512 : 256) / p.threads);
+    if (p.threads > 32) p.groups = std::min(p.groups, kMaxGroups<kStreams>);
+    while (p.groups > 1 && least * row_stage * p.groups > ring_smem(kStreams)) p.groups /= 2;
+    const int stage = row_stage * p.groups;
     p.blocks_per_sm = std::max(1, std::min(kRingThreads / (p.threads * p.groups), ring_smem(kStreams) / (least * stage)));
     p.stages = std::min(kRingStages, std::max(1, ring_smem(kStreams) / p.blocks_per_sm / stage));
-    p.smem = std::max(p.stages * stage, p.groups > 1 ? static_cast<int>(8 * C) : 0);
+    p.smem = std::max(p.stages * stage, Shape<kStreams, 0>::kSums ? p.groups * 8 * part_pitch(static_cast<int>(C)) : 0);
     if (stage > kMostSmem) p.stages = 0;
     return p;
 }

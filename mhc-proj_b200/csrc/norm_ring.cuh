@@ -33,11 +33,19 @@ namespace mhcp {
 
 constexpr int kRingThreads = 512;  // of an SM, in its rings' blocks
 
+// Groups of more than a warp in a block, at most (the memory for their sums).
+template <int kStreams>
+constexpr int kMaxGroups = kStreams == 1 ? 8 : 4;
+
 // Bytes of one row's place in a stage.
 __host__ __device__ inline int ring_row_bytes(int C, int elem, bool loose, int threads, int per_thread)
 {
     return loose ? (C * elem + 15) / 16 * 16 + 16 : threads * per_thread * elem;
 }
+
+// Floats of a row of partial sums in shared memory: the columns, from the start of
+// a skewed row's first piece, in whole pieces.
+__host__ __device__ inline int part_pitch(int C) { return (C + 15) / 8 * 8; }
 
 // The ring of one group: kRows rows a stage, kElems elements of a row a thread.
 template <class Elem, int kRows, RowForm kForm, int kElems>
@@ -133,7 +141,7 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
               float* __restrict__ mean_out, float* __restrict__ rstd_out, float eps, int64_t N, int C, int stages)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ __align__(16) float buf[kMaxGroups][2][kTurn * 32];
+    __shared__ __align__(16) float buf[kMaxGroups<kStreams>][2][kTurn * 32];
     using Ring = RowRing<Elem, kStreams * kTurn, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
     const Group group;
@@ -304,7 +312,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
 {
     extern __shared__ __align__(16) char ring_memory[];
     constexpr int kSums = kStreams == 1 ? 2 : 16;
-    __shared__ __align__(16) float buf[kMaxGroups][2][kSums * 32];
+    __shared__ __align__(16) float buf[kMaxGroups<kStreams>][2][kSums * 32];
     constexpr int kRows = kStreams + 1;  // of a stage: the streams, then g
     using Ring = RowRing<Elem, kRows, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
@@ -524,39 +532,43 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
         parity ^= 1;
     }
     if (!partials) return;
-    float* out = partials + static_cast<int64_t>(blockIdx.x) * 2 * C;
-    if (blockDim.y > 1) {
-        // the groups' parts, added one group after another
-        float* sum = reinterpret_cast<float*>(ring_memory);
-        for (int k = 0; k < static_cast<int>(blockDim.y); ++k) {
-            __syncthreads();
-            if (static_cast<int>(threadIdx.y) != k) continue;
+    // The groups' parts go through shared memory: one row of the workspace a
+    // block, written in whole lines.  A skewed row's pieces keep their places.
+    int2 me, of;  // read again: kept through the loop they cost registers that it has not
+    asm volatile("mov.u32 %0, %%tid.x; mov.u32 %1, %%tid.y;" : "=r"(me.x), "=r"(me.y));
+    asm volatile("mov.u32 %0, %%ntid.x; mov.u32 %1, %%ntid.y;" : "=r"(of.x), "=r"(of.y));
+    float* part = reinterpret_cast<float*>(ring_memory) + static_cast<size_t>(me.y) * 2 * part_pitch(C);
+    __syncthreads();  // the rings have been read
+    auto put = [&](float* to, int p, const float2 (&v)[K / 2]) {
+        if constexpr (kForm == kLoose) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
+            for (int j = 0; j < K; ++j)
+                if (cols.in(p, j)) to[cols.col(p, j)] = j & 1 ? v[j / 2].y : v[j / 2].x;
+        } else if (cols.has(p)) {
 #pragma unroll
-                for (int j = 0; j < K; ++j) {
-                    if (!cols.in(p, j)) continue;
-                    const int c = cols.col(p, j);
-                    float &a = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x, &b = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
-                    if (k > 0) {
-                        a += sum[c];
-                        b += sum[C + c];
-                    }
-                    sum[c] = a;
-                    sum[C + c] = b;
-                }
-            }
+            for (int j = 0; j < K / 2; j += 2)
+                *reinterpret_cast<float4*>(to + ring.piece(p) * K + 2 * j) = make_float4(v[j].x, v[j].y, v[j + 1].x, v[j + 1].y);
         }
-        if (static_cast<int>(threadIdx.y) != static_cast<int>(blockDim.y) - 1) return;
-    }
+    };
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (!cols.in(p, j)) continue;
-            out[cols.col(p, j)] = j & 1 ? dw[p][j / 2].y : dw[p][j / 2].x;
-            out[C + cols.col(p, j)] = j & 1 ? db[p][j / 2].y : db[p][j / 2].x;
+        put(part, p, dw[p]);
+        put(part + part_pitch(C), p, db[p]);
+    }
+    __syncthreads();
+    float* out = partials + static_cast<int64_t>(blockIdx.x) * 2 * C;
+    const float* from = reinterpret_cast<const float*>(ring_memory);
+    for (int c = me.y * of.x + me.x; c < C; c += of.x * of.y) {
+        float w = 0.0f, b = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < of.y; ++k) {
+            const int64_t r = blockIdx.x * static_cast<int64_t>(of.y) + k;
+            const float* at = from + k * 2 * part_pitch(C) + c + row_skew<Elem, kForm>(src.x + r * src.stride);
+            w += at[0];
+            b += at[part_pitch(C)];
         }
+        out[c] = w;
+        out[C + c] = b;
     }
 }
 

@@ -127,8 +127,6 @@ struct Group {
     }
 };
 
-constexpr int kMaxGroups = 4;  // of more than a warp, in a block
-
 // Sums of K values over a group's threads, in every thread, in an order fixed
 // by the group's size.  `buf`: 32 K floats of the group at a 16-byte boundary
 // that group_sum_init has seen; the caller keeps two calls with the same buf
