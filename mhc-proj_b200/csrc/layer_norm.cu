@@ -86,8 +86,10 @@ static cudaError_t by_form(RowForm form, Launch launch)
 
 // The ring kernels' shapes by width: elements of a row per thread, the most
 // threads of a group (their product is the widest row), rows a turn, and
-// whether the parameters stay in registers.  All are within 128 registers a
-// thread; a spill costs more than what the held values save.
+// whether the parameters stay in registers.  512 threads of an SM have 128
+// registers each: the shapes of the widths up to 4096 fit in them but for a
+// pair (16 elements a thread for the four streams' gradients, which spill: 506 us
+// against 440, 65536 x 2048 bf16); wider rows spill what 32 elements a thread need.
 template <int kStreams, int kWidth>
 struct FwdShape {
     static constexpr int kElems = kWidth ? 32 : 16, kTurn = kStreams == 1 && !kWidth ? 2 : 1;
@@ -154,10 +156,12 @@ static RingPlan ring_plan(int64_t C, int elem, RowForm form)
     p.form = form == kPieces && p.threads * p.elems == C ? kWhole : form;
     const int row_stage = rows * ring_row_bytes(static_cast<int>(C), elem, form == kLoose, p.threads, p.elems);
     const int least = kStreams == 1 ? 1 : 2;  // stages
-    // The sums' rows of two blocks an SM cost skewed rows more than their waits for
-    // one another in one block (backward, bf16, 20003 x 1025: 57 us in blocks of 512
-    // threads, 61 of 256; whole pieces, 65536 x 4096: 269 and 263).
-    p.groups = std::max(1, (Shape<kStreams, 0>::kSums && form == kSkewed ? 512 : 256) / p.threads);
+    // Blocks of about 256 threads, or of up to 512 where two of the smaller leave
+    // threads of the SM without work (groups of 96, bf16, 20003 x 1025: forward 39
+    // us in blocks of five, 43 in two of two; backward 57 and 61.  65536 x 4096
+    // backward, as many threads either way: 269 in one block, 263 in two).
+    p.groups = std::max(1, 256 / p.threads);
+    if (kRingThreads / p.threads > kRingThreads / (p.threads * p.groups) * p.groups) p.groups = kRingThreads / p.threads;
     if (p.threads > 32) p.groups = std::min(p.groups, kMaxGroups<kStreams>);
     while (p.groups > 1 && least * row_stage * p.groups > ring_smem(kStreams)) p.groups /= 2;
     const int stage = row_stage * p.groups;

@@ -18,11 +18,12 @@
 // registers, and the parameters stay in registers over all rows.  Forward, 65536
 // x 4096 bf16: 168 us, 6.4 TB/s (a block per row with the row in registers 342;
 // the ring with the parameters read for each row 283).  The backward pass has
-// three tensors and twice the sums: 258 us, 6.2 TB/s (1762 with three readings
+// three tensors and twice the sums: 251 us, 6.4 TB/s (1762 with three readings
 // and separate sums of the parameters' gradients; the ring alone 393, with
 // packed arithmetic 320, with the parameters held 303, with the pieces held as
-// they are so that a stage is refilled at once 264).  Under a load of seconds
-// the clock falls and its instructions show: 287 us.
+// they are so that a stage is refilled at once 264, with blocks' sums in whole
+// lines 251).  Under a load of seconds the clock falls and its instructions
+// show: 283 us.
 #pragma once
 
 #include "norm_source.cuh"
@@ -35,7 +36,7 @@ constexpr int kRingThreads = 512;  // of an SM, in its rings' blocks
 
 // Groups of more than a warp in a block, at most (the memory for their sums).
 template <int kStreams>
-constexpr int kMaxGroups = kStreams == 1 ? 8 : 4;
+constexpr int kMaxGroups = kStreams == 1 ? 8 : 5;
 
 // Bytes of one row's place in a stage.
 __host__ __device__ inline int ring_row_bytes(int C, int elem, bool loose, int threads, int per_thread)

@@ -81,7 +81,7 @@ inline int sm_count()
     return sms;
 }
 
-// The dynamic shared memory of a launch at most; the kernels' static memory (16
+// The dynamic shared memory of a launch at most; the kernels' static memory (20
 // KB at most) fits beside it.
 constexpr int kMostSmem = 200 * 1024;
 
