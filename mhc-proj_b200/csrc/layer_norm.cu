@@ -163,6 +163,7 @@ static RingPlan ring_plan(int64_t C, int elem, RowForm form)
     p.groups = std::max(1, 256 / p.threads);
     if (kRingThreads / p.threads > kRingThreads / (p.threads * p.groups) * p.groups) p.groups = kRingThreads / p.threads;
     if (p.threads > 32) p.groups = std::min(p.groups, kMaxGroups<kStreams>);
+    // two stages of all groups' rows have to fit (four streams in fp32)
     while (p.groups > 1 && least * row_stage * p.groups > ring_smem(kStreams)) p.groups /= 2;
     const int stage = row_stage * p.groups;
     p.blocks_per_sm = std::max(1, std::min(kRingThreads / (p.threads * p.groups), ring_smem(kStreams) / (least * stage)));
