@@ -84,95 +84,6 @@ static cudaError_t by_form(RowForm form, Launch launch)
     return launch(std::integral_constant<RowForm, kLoose>{});
 }
 
-// The ring kernels' shapes by width: elements of a row per thread, the most
-// threads of a group (their product is the widest row), rows a turn, and
-// whether the parameters stay in registers.  512 threads of an SM have 128
-// registers each: the shapes of the widths up to 4096 fit in them but for a
-// pair (16 elements a thread for the four streams' gradients, which spill: 506 us
-// against 440, 65536 x 2048 bf16); wider rows spill what 32 elements a thread need.
-template <int kStreams, int kWidth>
-struct FwdShape {
-    static constexpr int kElems = kWidth ? 32 : 16, kTurn = kStreams == 1 && !kWidth ? 2 : 1;
-    static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
-    static constexpr bool kHold = true;
-    static constexpr int kRows = kStreams * kTurn;  // of a stage
-    static constexpr bool kSums = false;            // of the parameters' gradients, in shared memory at the end
-    static constexpr int64_t kWidest = kElems * kMaxThreads;
-};
-template <int kStreams, int kWidth>
-struct BwdShape {
-    static constexpr int kElems = kWidth == 2 ? 32 : kStreams == 1 || kWidth == 1 ? 16 : 8;
-    static constexpr int kMaxThreads = kStreams == 1 && !kWidth ? 256 : 512;
-    static constexpr bool kHold = kWidth == 0 || (kStreams == 1 && kWidth == 1);
-    static constexpr int kRows = kStreams + 1;
-    static constexpr bool kSums = true;
-    static constexpr int64_t kWidest = kElems * kMaxThreads;
-};
-
-// A ring kernel's launch.
-struct RingPlan {
-    RowForm form;
-    int width, elems, threads, groups, stages, blocks_per_sm, smem;
-
-    // Blocks for `turns` turns of the groups.
-    int64_t grid(int64_t turns, int elem) const
-    {
-        const int64_t blocks = std::min(ceil_div(turns, groups), static_cast<int64_t>(blocks_per_sm) * sm_count());
-        if (form != kSkewed) return blocks;
-        // the groups' turns go in steps of whole periods of 16 / elem rows
-        const int period = 16 / elem, unit = period / std::min(period, groups & -groups);
-        return std::max<int64_t>(unit, blocks / unit * unit);
-    }
-};
-
-// Of an SM's 227 KB, for the rings: more bytes under way are slower again (one
-// stream, fp32, 16384 x 4096 forward: 100 KB 90 us, 204 KB 98; four streams, fp32,
-// 16384 x 2048 backward: 150 KB 184 us, 204 KB 219).
-constexpr int ring_smem(int streams) { return (streams == 1 ? 100 : 150) * 1024; }
-
-// The shape (of kWidths) and launch for rows of C elements in `form`; stages 0: too wide.
-template <template <int, int> class Shape, int kStreams, int kWidths>
-static RingPlan ring_plan(int64_t C, int elem, RowForm form)
-{
-    RingPlan p{};
-    const int64_t span = C + (form == kSkewed ? 16 / elem - 1 : 0);  // columns from a piece's start
-    if (span > Shape<kStreams, kWidths - 1>::kWidest) return p;
-    int rows = Shape<kStreams, 0>::kRows;
-    p.elems = Shape<kStreams, 0>::kElems;
-    if (span > Shape<kStreams, 0>::kWidest) {
-        p.width = 1;
-        rows = Shape<kStreams, 1>::kRows;
-        p.elems = Shape<kStreams, 1>::kElems;
-    }
-    if (kWidths > 2 && span > Shape<kStreams, 1>::kWidest) {
-        p.width = 2;
-        rows = Shape<kStreams, kWidths - 1>::kRows;
-        p.elems = Shape<kStreams, kWidths - 1>::kElems;
-    }
-    const int64_t want = ceil_div(span, p.elems);
-    p.threads = form == kLoose ? 32 : 4;
-    while (p.threads < 32 && p.threads < want) p.threads *= 2;
-    if (want > 32) p.threads = 32 * static_cast<int>(ceil_div(want, 32));
-    p.form = form == kPieces && p.threads * p.elems == C ? kWhole : form;
-    const int row_stage = rows * ring_row_bytes(static_cast<int>(C), elem, form == kLoose, p.threads, p.elems);
-    const int least = kStreams == 1 ? 1 : 2;  // stages
-    // Blocks of about 256 threads, or of up to 512 where two of the smaller leave
-    // threads of the SM without work (groups of 96, bf16, 20003 x 1025: forward 39
-    // us in blocks of five, 43 in two of two; backward 57 and 61.  65536 x 4096
-    // backward, as many threads either way: 269 in one block, 263 in two).
-    p.groups = std::max(1, 256 / p.threads);
-    if (kRingThreads / p.threads > kRingThreads / (p.threads * p.groups) * p.groups) p.groups = kRingThreads / p.threads;
-    if (p.threads > 32) p.groups = std::min(p.groups, kMaxGroups<kStreams>);
-    // two stages of all groups' rows have to fit (four streams in fp32)
-    while (p.groups > 1 && least * row_stage * p.groups > ring_smem(kStreams)) p.groups /= 2;
-    const int stage = row_stage * p.groups;
-    p.blocks_per_sm = std::max(1, std::min(kRingThreads / (p.threads * p.groups), ring_smem(kStreams) / (least * stage)));
-    p.stages = std::min(kRingStages, std::max(1, ring_smem(kStreams) / p.blocks_per_sm / stage));
-    p.smem = std::max(p.stages * stage, Shape<kStreams, 0>::kSums ? p.groups * 8 * part_pitch(static_cast<int>(C)) : 0);
-    if (stage > kMostSmem) p.stages = 0;
-    return p;
-}
-
 template <class Elem, int kStreams, RowForm kForm, int kWidth>
 static cudaError_t norm_forward_ring(const RingPlan& p, const NormSource<Elem, kStreams>& src, const NormAffine& aff,
                                      Elem* y, float* mean, float* rstd, float eps, int64_t N, int64_t C,
@@ -180,9 +91,10 @@ static cudaError_t norm_forward_ring(const RingPlan& p, const NormSource<Elem, k
 {
     using S = FwdShape<kStreams, kWidth>;
     const auto kernel = norm_fwd_ring<Elem, kStreams, kForm, S::kElems, S::kTurn, S::kHold>;
-    const cudaError_t e = allow_smem(kernel, p.smem);
+    const cudaError_t e = allow_smem<sizeof(typename S::Sums)>(kernel, p.smem);
     if (e != cudaSuccess) return e;
-    kernel<<<static_cast<unsigned>(p.grid(ceil_div(N, S::kTurn), sizeof(Elem))), dim3(p.threads, p.groups), p.smem, stream>>>(
+    const int64_t grid = p.grid(ceil_div(N, S::kTurn), sizeof(Elem), sm_count());
+    kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
         src, span_of(src.x, N, src.stride, kStreams, src.stream_stride, C), aff, y, mean, rstd, eps, N,
         static_cast<int>(C), p.stages);
     return cudaSuccess;
@@ -250,7 +162,7 @@ static cudaError_t norm_backward_ring(const RingPlan& p, int64_t grid, const Ele
 {
     using S = BwdShape<kStreams, kWidth>;
     const auto kernel = norm_bwd_ring<Elem, kStreams, kForm, S::kElems, S::kHold>;
-    const cudaError_t e = allow_smem(kernel, p.smem);
+    const cudaError_t e = allow_smem<sizeof(typename S::Sums)>(kernel, p.smem);
     if (e != cudaSuccess) return e;
     kernel<<<static_cast<unsigned>(grid), dim3(p.threads, p.groups), p.smem, stream>>>(
         g, g_stride, span_of(g, N, g_stride, 1, 0, C), src,
@@ -293,7 +205,7 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
     const RingPlan plan = ring_plan<BwdShape, kStreams, 3>(C, sizeof(Elem), form);
     int64_t rows = 0;  // of partial sums
     if (N > 0 && plan.stages > 0) {
-        rows = std::min(plan.grid(N, sizeof(Elem)), kMaxPartials);
+        rows = std::min(plan.grid(N, sizeof(Elem), sm_count()), kMaxPartials);
         const cudaError_t e = by_form<kStreams>(plan.form, [&](auto f) {
             constexpr RowForm form = decltype(f)::value;
             switch (plan.width) {

@@ -26,6 +26,11 @@ constexpr int kMixRingBlock = 128;
 // (forward 4 stages: 429 us for 375) meet one another in the memory system.
 constexpr int kMixFwdStages = 2, kMixBwdStages = 2, kMixFwdBlocks = 4;
 
+// What of a chunk is kept, by warp: the ring kernels' static memory.
+struct MixMasks {
+    alignas(16) unsigned char of[kMixRingBlock / 32][32];
+};
+
 template <class Elem, bool kVec>
 struct MixChunk {
     static constexpr int K = 16 / sizeof(Elem);
@@ -175,7 +180,7 @@ __global__ void __launch_bounds__(kMixRingBlock)
 mix_fwd_ring(MixIn<Elem> in, RowSpan x_span, RowSpan y_span, Elem* __restrict__ out, Dropout d, int64_t N, int C, int lanes)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ __align__(16) unsigned char masks[kMixRingBlock / 32][32];
+    __shared__ MixMasks masks;
     using Chunk = MixChunk<Elem, kVec>;
     constexpr int kPairs = Chunk::kPairs, kPlace = Chunk::kPlace;
     constexpr int kStage = 5 * kPlace;
@@ -223,7 +228,7 @@ mix_fwd_ring(MixIn<Elem> in, RowSpan x_span, RowSpan y_span, Elem* __restrict__ 
 #pragma unroll
         for (int j = 0; j < 4; ++j) at_x[j] = ch.at(place + j * kPlace, in.x + r * in.stride + j * in.stream_stride, c);
         typename Chunk::Keep keep;
-        if (d.limit) keep = ch.keep(r * C, c, d, key, masks[warp]);
+        if (d.limit) keep = ch.keep(r * C, c, d, key, masks.of[warp]);
         Elem* to = out + r * 4 * C + c;
         const int steps = ch.steps(c);
 #pragma unroll
@@ -265,7 +270,7 @@ mix_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stri
              void* __restrict__ dh, Dropout d, int64_t N, int C, int lanes)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ __align__(16) unsigned char masks[kMixRingBlock / 32][32];
+    __shared__ MixMasks masks;
     using Chunk = MixChunk<Elem, kVec>;
     constexpr int kPairs = Chunk::kPairs, kPlace = Chunk::kPlace;
     constexpr int kStage = 9 * kPlace;
@@ -320,7 +325,7 @@ mix_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stri
                 at_g[j] = ch.at(place + (5 + j) * kPlace, g + r * g_stride + j * g_stream_stride, c);
             }
             typename Chunk::Keep keep;
-            if (d.limit) keep = ch.keep(r * C, c, d, key, masks[warp]);
+            if (d.limit) keep = ch.keep(r * C, c, d, key, masks.of[warp]);
             Elem *to = dx + r * 4 * C + c, *to_y = dy + r * C + c;
             const int steps = ch.steps(c);
 #pragma unroll

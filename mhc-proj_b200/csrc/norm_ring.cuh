@@ -27,26 +27,11 @@
 #pragma once
 
 #include "norm_source.cuh"
+#include "ring_plan.h"
 #include "row_cols.cuh"
 #include "row_copy.cuh"
 
 namespace mhcp {
-
-constexpr int kRingThreads = 512;  // of an SM, in its rings' blocks
-
-// Groups of more than a warp in a block, at most (the memory for their sums).
-template <int kStreams>
-constexpr int kMaxGroups = kStreams == 1 ? 8 : 5;
-
-// Bytes of one row's place in a stage.
-__host__ __device__ inline int ring_row_bytes(int C, int elem, bool loose, int threads, int per_thread)
-{
-    return loose ? (C * elem + 15) / 16 * 16 + 16 : threads * per_thread * elem;
-}
-
-// Floats of a row of partial sums in shared memory: the columns, from the start of
-// a skewed row's first piece, in whole pieces.
-__host__ __device__ inline int part_pitch(int C) { return (C + 15) / 8 * 8; }
 
 // The ring of one group: kRows rows a stage, kElems elements of a row a thread.
 template <class Elem, int kRows, RowForm kForm, int kElems>
@@ -142,7 +127,7 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
               float* __restrict__ mean_out, float* __restrict__ rstd_out, float eps, int64_t N, int C, int stages)
 {
     extern __shared__ __align__(16) char ring_memory[];
-    __shared__ __align__(16) float buf[kMaxGroups<kStreams>][2][kTurn * 32];
+    __shared__ GroupSums<kStreams, kTurn> buf;
     using Ring = RowRing<Elem, kStreams * kTurn, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
     const Group group;
@@ -154,7 +139,7 @@ norm_fwd_ring(NormSource<Elem, kStreams> src, RowSpan span, NormAffine aff, Elem
     const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm == kLoose, group.threads, kElems);
     const typename Ring::Cols cols(C, group.t, group.threads, row_skew<Elem, kForm>(src.x + row_of(first, 0) * src.stride));
     const Ring ring{ring_memory + static_cast<size_t>(group.id) * stages * kStreams * kTurn * row_bytes, row_bytes, cols};
-    float(*sums)[kTurn * 32] = buf[group.one_warp() ? 0 : group.id];  // a warp's group needs none
+    float(*sums)[kTurn * 32] = buf.of[group.one_warp() ? 0 : group.id];  // a warp's group needs none
     group_sum_init<kTurn>(group, sums[0]);
     group_sum_init<kTurn>(group, sums[1]);
     auto fill = [&](int stage, int64_t turn) {
@@ -313,7 +298,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
 {
     extern __shared__ __align__(16) char ring_memory[];
     constexpr int kSums = kStreams == 1 ? 2 : 16;
-    __shared__ __align__(16) float buf[kMaxGroups<kStreams>][2][kSums * 32];
+    __shared__ GroupSums<kStreams, kSums> buf;
     constexpr int kRows = kStreams + 1;  // of a stage: the streams, then g
     using Ring = RowRing<Elem, kRows, kForm, kElems>;
     constexpr int K = Ring::K, P = Ring::P;
@@ -323,7 +308,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
     const int row_bytes = ring_row_bytes(C, sizeof(Elem), kForm == kLoose, group.threads, kElems);
     const typename Ring::Cols cols(C, group.t, group.threads, row_skew<Elem, kForm>(src.x + first * src.stride));
     const Ring ring{ring_memory + static_cast<size_t>(group.id) * stages * kRows * row_bytes, row_bytes, cols};
-    float(*sums)[kSums * 32] = buf[group.one_warp() ? 0 : group.id];  // a warp's group needs none
+    float(*sums)[kSums * 32] = buf.of[group.one_warp() ? 0 : group.id];  // a warp's group needs none
     group_sum_init<2>(group, sums[0]);
     group_sum_init<2>(group, sums[1]);
     auto fill = [&](int stage, int64_t r) {

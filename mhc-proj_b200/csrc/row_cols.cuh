@@ -12,11 +12,10 @@
 // written.
 #pragma once
 
+#include "ring_plan.h"
 #include "row_ops.cuh"
 
 namespace mhcp {
-
-enum RowForm { kLoose, kSkewed, kPieces, kWhole };
 
 // An array of Param at single columns of a thread.
 template <class Param, class Cols, int kPairs>

@@ -2,6 +2,7 @@
 // that hold no registers.
 #pragma once
 
+#include "ring_plan.h"
 #include "row_ops.cuh"
 
 namespace mhcp {
@@ -26,8 +27,6 @@ __device__ __forceinline__ void copies_wait(int stages)
     else
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
-
-constexpr int kRingStages = 4;  // at most
 
 // A tensor of rows: its bytes from the first to the last element, and whether
 // its rows follow one another at 32 bytes or more, so that around every row
@@ -81,19 +80,18 @@ inline int sm_count()
     return sms;
 }
 
-// The dynamic shared memory of a launch at most; the kernels' static memory (20
-// KB at most) fits beside it.
-constexpr int kMostSmem = 200 * 1024;
-
-// A launch may need more dynamic shared memory than a kernel has by default
-// (48 KB, less what is static).  The limit belongs to the kernel in the context
-// and not to the launch, so every launch sets the same one: two host threads
-// with rows of two widths do not undo each other's.
-template <class Kernel>
+// A launch may need more shared memory than a kernel has by default, which is
+// for its static memory too (a four-stream norm backward's 20 KB).  The limit belongs to
+// the kernel in the context and not to the launch, so every launch that has to
+// ask sets the same one: two host threads with rows of two widths do not undo
+// each other's.
+template <int kStaticBytes, class Kernel>
 inline cudaError_t allow_smem(Kernel kernel, int bytes)
 {
-    return bytes <= 32 * 1024 ? cudaSuccess
-                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    static_assert(kStaticBytes + kMostSmem <= kLargestSmem, "the static memory has to fit beside the rings");
+    return asks_for_smem(kStaticBytes, bytes)
+               ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)
+               : cudaSuccess;
 }
 
 }  // namespace mhcp

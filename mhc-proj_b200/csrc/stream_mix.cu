@@ -249,7 +249,7 @@ static int mix_forward_ring(const MixIn<Elem>& in, Elem* out, const Dropout& d, 
     using Chunk = MixChunk<Elem, kVec>;
     const int lanes = kVec ? mix_threads(C / Chunk::K, 1, 32) : 32;
     constexpr int warps = kMixRingBlock / 32, smem = warps * kMixFwdStages * 5 * Chunk::kPlace;
-    const cudaError_t e = allow_smem(mix_fwd_ring<Elem, kVec, kWide>, smem);
+    const cudaError_t e = allow_smem<sizeof(MixMasks)>(mix_fwd_ring<Elem, kVec, kWide>, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t items = ceil_div(N, 32 / lanes) * Chunk::count(static_cast<int>(C), lanes);
     const int64_t grid = std::min<int64_t>(ceil_div(items, warps), kMixFwdBlocks * sm_count());
@@ -277,7 +277,7 @@ static int mix_backward_ring(const Elem* g, int64_t g_stride, int64_t g_stream_s
 {
     using Chunk = MixChunk<Elem, kVec>;
     constexpr int warps = kMixRingBlock / 32, smem = warps * kMixBwdStages * 9 * Chunk::kPlace;
-    const cudaError_t e = allow_smem(mix_bwd_ring<Elem, kVec, kWide>, smem);
+    const cudaError_t e = allow_smem<sizeof(MixMasks)>(mix_bwd_ring<Elem, kVec, kWide>, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int lanes = kVec ? mix_threads(C / Chunk::K, 1, 32) : 32;
     // Two blocks an SM (65536 tokens of 2048, bf16: 595 us, with three 675), or
