@@ -18,7 +18,7 @@
 // registers, and the parameters stay in registers over all rows.  Forward, 65536
 // x 4096 bf16: 168 us, 6.4 TB/s (a block per row with the row in registers 342;
 // the ring with the parameters read for each row 283).  The backward pass has
-// three tensors and twice the sums: 251 us, 6.4 TB/s (1762 with three readings
+// three tensors and twice the sums: 252 us, 6.4 TB/s (1762 with three readings
 // and separate sums of the parameters' gradients; the ring alone 393, with
 // packed arithmetic 320, with the parameters held 303, with the pieces held as
 // they are so that a stage is refilled at once 264, with blocks' sums in whole
@@ -281,13 +281,19 @@ __device__ __forceinline__ float warp_sum16(float (&v)[16])
 // registers over all its rows: partials[block][0 or 1][C] (null: neither is
 // wanted).
 //
+// xhat is formed from the distance u - mean.  u rstd - (mean rstd) would be one
+// operation a pair of columns less (250 us for 252, 65536 x 4096 bf16; four
+// streams, 65536 x 1024 fp16, 203 for 205), but the product's rounding is an error
+// of all of a row's xhat that grows with |mean| rstd: 6e-5 at a centre 1024
+// times the spread, and a gradient for the weight from rows of one value.
+//
 // All that a row's gradients need is summed in one go over the row, so that
 // its stage is free again before the sums are known: sum(gw) and
 // sum(gw xhat), and for the streams' weights
 //   dh[i] = sum(du X[i]) = rstd (sum(gw X[i]) - m1 sum(X[i]) - m2 sum(xhat X[i])),
 // m1 = sum(gw) / C, m2 = sum(gw xhat) / C.  A thread keeps its elements' gw and
 // xhat until then (of one stream: the 16-byte pieces of g and x as they are).
-// Four streams, 65536 x 2048 bf16: 390 us, 6.2 TB/s, 438 under a load of seconds
+// Four streams, 65536 x 2048 bf16: 400 us, 6.0 TB/s, 447 under a load of seconds
 // (498 with dh in a second pass over the stage, 506 with 16 elements a thread,
 // which spill).
 template <class Elem, int kStreams, RowForm kForm, int kElems, bool kHold>
@@ -377,7 +383,6 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                     ring.get(stage, 1, p, gr, gv);
                 }
             };
-            const float shift = -mean * rstd;  // xhat = u rstd + shift
             float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -386,7 +391,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 weight(p, w);
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j) {  // g is zero beyond the row
-                    const float2 xhat = fma2(u[j], both(rstd), both(shift));
+                    const float2 xhat = mul2(add2(u[j], both(-mean)), both(rstd));
                     const float2 gw = mul2(gv[j], w[j]);
                     s0 = add2(s0, gw);
                     s1 = fma2(gw, xhat, s1);
@@ -396,9 +401,8 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
             }
             float s[2] = {s0.x + s0.y, s1.x + s1.y};
             group_sum(group, s, sums[parity]);
-            // du = rstd (gw - m1 - xhat m2) = g (w rstd) + (u slope + level)
-            const float m1 = s[0] * inv, m2 = s[1] * inv;
-            const float slope = -rstd * rstd * m2, level = -rstd * (m1 + shift * m2);
+            // du = rstd (gw - m1 - (u - mean) rstd m2)
+            const float m1 = s[0] * inv, m2 = -s[1] * inv * rstd;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 float2 du[K / 2], u[K / 2], w[K / 2];
@@ -406,7 +410,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 weight(p, w);
 #pragma unroll
                 for (int j = 0; j < K / 2; ++j)
-                    du[j] = fma2(du[j], mul2(w[j], both(rstd)), fma2(u[j], both(slope), both(level)));
+                    du[j] = mul2(both(rstd), fma2(add2(u[j], both(-mean)), both(m2), fma2(du[j], w[j], both(-m1))));
                 cols.store(p, dx + r * C, du);
             }
             if constexpr (kForm == kLoose) {
@@ -414,7 +418,6 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                 fill(stage, r + stages * step);
             }
         } else {
-            const float shift = -mean * rstd;  // xhat = u rstd + shift
             float2 gw[P][K / 2], xhat[P][K / 2];
             float2 s0 = both(0.0f), s1 = both(0.0f), sx[kStreams], sg[kStreams], sh[kStreams];
 #pragma unroll
@@ -431,7 +434,7 @@ norm_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, RowSpan g_span, Norm
                     float2 u = mul2(v[0][j], both(row.h[0]));
 #pragma unroll
                     for (int i = 1; i < kStreams; ++i) u = fma2(v[i][j], both(row.h[i]), u);
-                    const float2 x = fma2(u, both(rstd), both(shift)), y = mul2(gv[j], w[j]);
+                    const float2 x = mul2(add2(u, both(-mean)), both(rstd)), y = mul2(gv[j], w[j]);
                     s0 = add2(s0, y);
                     s1 = fma2(y, x, s1);
                     dw[p][j] = fma2(gv[j], x, dw[p][j]);

@@ -58,3 +58,102 @@ def test_a_process_may_begin_with_any_width():
     with ThreadPoolExecutor(4) as pool:
         got = dict(zip(FIRST, pool.map(first_call, FIRST)))
     assert {k: v for k, v in got.items() if v != "ok"} == {}
+
+
+# ---- rows far from zero ----------------------------------------------------------------
+
+def near_backward(g, u, u_off, mean, rstd, weight, bias, depth, rows_depth):
+    """residual_reference.norm_backward with the bound of an evaluation that
+    takes the distance u - mean before it multiplies.  The statistics are
+    given, so the distance is rounded relative to itself and xhat = (u - mean)
+    rstd is off by 2 * 2^-24 |xhat|, and by `u_off` * 2^-24 * rstd where u is
+    itself a rounded sum (its roundings times the sum of its terms' sizes).
+    Neither grows with |mean|.  The roundings per term (at most 8) are among
+    `depth` (at least 33)."""
+    g, mean, rstd = g.double(), mean.double()[:, None], rstd.double()[:, None]
+    one = torch.ones(u.shape[-1], dtype=torch.float64, device=u.device)
+    w = one if weight is None else weight.double()
+    xhat = (u - mean) * rstd
+    xhat_off = u_off * rstd / depth
+    gw = g * w
+    m2, m2_mag = (gw * xhat).mean(-1, keepdim=True), (gw.abs() * (xhat.abs() + xhat_off)).mean(-1, keepdim=True)
+    du = rstd * (gw - gw.mean(-1, keepdim=True) - xhat * m2)
+    du_mag = rstd * (gw.abs() + gw.abs().mean(-1, keepdim=True) + (xhat.abs() + xhat_off) * m2_mag)
+    out = {"du": (du, du_mag, depth)}
+    if weight is not None:
+        xhat_off = u_off * rstd / rows_depth
+        out["d_weight"] = ((g * xhat).sum(0), (g.abs() * (xhat.abs() + xhat_off)).sum(0), rows_depth)
+    if bias is not None:
+        out["d_bias"] = (g.sum(0), g.abs().sum(0), rows_depth)
+    return out
+
+
+def near_layer_norm(G, x, mean, rstd, w, b, depth=None):
+    out = near_backward(G, x.double(), 0.0, mean, rstd, w, b, depth or ref.row_depth(x.shape[-1]),
+                        ref.rows_depth(len(x)))
+    out["d_x"] = out.pop("du")
+    return out
+
+
+def near_stream_norm(G, X, h, mean, rstd, w, b, depth=None):
+    u, mag = ref.read(X, h)
+    D = depth or ref.row_depth(X.shape[-1])
+    out = near_backward(G, u, 4 * mag, mean, rstd, w, b, D, ref.rows_depth(len(X)))
+    du, du_mag, _ = out.pop("du")
+    X, h = X.double(), h.double()
+    out["d_X"] = (h[:, :, None] * du[:, None], h.abs()[:, :, None] * du_mag[:, None], D)
+    out["d_h_pre"] = ((X * du[:, None]).sum(-1), (X.abs() * du_mag[:, None]).sum(-1), 2 * D)
+    return out
+
+
+@pytest.mark.parametrize("C", [7, 128, 1001, 4096, 5000, 9000, 20001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_gradients_of_rows_far_from_zero(dtype, C):
+    """Centres of 2^10 and -2^9 under a spread of 1 to 8: a product mean * rstd
+    rounded before the difference is taken puts 2^-24 * 2^10 on all of a row's
+    xhat, where the distance from the mean has 2^-24 * |xhat|."""
+    g = gen(C + 70)
+    for N in (9, 300):
+        centre = torch.where(torch.arange(N, device="cuda") % 2 == 0, 1024.0, -512.0)
+        x, G = (8 * normal(g, N, C) + centre[:, None]).to(dtype), normal(g, N, C).to(dtype)
+        w, b = affine_of("float32", C, g, dtype)
+        out = f.layer_norm(x, w, b, EPS)
+        got = f.layer_norm_backward(G, x, out["mean"], out["rstd"], w, b)
+        ref.check(got, near_layer_norm(G, x, out["mean"], out["rstd"], w, b), (dtype, N, C))
+        X = (8 * normal(g, N, 4, C) + centre[:, None, None]).to(dtype)
+        h = torch.sigmoid(normal(g, N, 4))
+        out = f.stream_norm_n4(X, h, w, b, EPS)
+        got = f.stream_norm_n4_backward(G, X, h, out["mean"], out["rstd"], w, b)
+        ref.check(got, near_stream_norm(G, X, h, out["mean"], out["rstd"], w, b), (dtype, N, C, "streams"))
+
+
+@pytest.mark.parametrize("C", [8, 100, 1001, 4096, 9000, 20001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_at_their_mean_give_the_weight_no_gradient(dtype, C):
+    """u = mean in every column: xhat is zero, and so is d_weight, exactly."""
+    g = gen(C + 71)
+    N = 37
+    G, w = normal(g, N, C).to(dtype), 1 + 0.3 * normal(g, C)
+    mean, rstd = torch.full((N,), 100.0, device="cuda"), torch.full((N,), EPS ** -0.5, device="cuda")
+    x = torch.full((N, C), 100.0, device="cuda", dtype=dtype)
+    got = f.layer_norm_backward(G, x, mean, rstd, w, w)
+    assert not bool(got["d_weight"].any())
+    ref.check(got, near_layer_norm(G, x, mean, rstd, w, w), (dtype, C))
+    X, h = x[:, None].expand(N, 4, C), torch.full((N, 4), 0.25, device="cuda")
+    got = f.stream_norm_n4_backward(G, X, h, mean, rstd, w, w)
+    assert not bool(got["d_weight"].any())
+
+
+def test_norm_gradients_of_tiny_and_huge_spreads():
+    """rstd of 2^66 and 2^-60 in fp32: its square is no fp32 number, or a subnormal one."""
+    g = gen(72)
+    for C in (96, 4096, 20001):
+        for size in (2.0 ** -66, 2.0 ** 60):
+            x, G = normal(g, 5, C) * size, normal(g, 5, C)
+            w, b = affine_of("float32", C, g, torch.float32)
+            mean, rstd = torch.zeros(5, device="cuda"), torch.full((5,), 1 / size, device="cuda")
+            got = f.layer_norm_backward(G, x, mean, rstd, w, b)
+            ref.check(got, near_layer_norm(G, x, mean, rstd, w, b), (C, size))
+            X, h = normal(g, 5, 4, C) * size, torch.rand(5, 4, device="cuda", generator=g)
+            got = f.stream_norm_n4_backward(G, X, h, mean, rstd, w, b)
+            ref.check(got, near_stream_norm(G, X, h, mean, rstd, w, b), (C, size, "streams"))
