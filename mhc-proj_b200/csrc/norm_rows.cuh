@@ -1,6 +1,9 @@
-// Layer norm kernels for rows that the ring kernels do not hold (wider than
-// 16384 elements), one block per row in loops over its columns, and the fold
-// of the parameters' partial sums.
+// Layer norm kernels for rows that the ring kernels do not hold, one block per
+// row in loops over its columns, and the fold of the parameters' partial sums.
+// Such rows are wider than 16384 elements; in the backward also skewed ones from
+// 16378 (fp32 16382), and four streams in fp32 from 10244 (loose ones 10237), a
+// stage of which does not fit in a block's shared memory.  Bound by latency:
+// every pass reads single elements, from L1 or L2 after the first.
 #pragma once
 
 #include "norm_source.cuh"
@@ -8,6 +11,29 @@
 namespace mhcp {
 
 constexpr int kNormBlock = 256;
+
+// Adds up a thread's columns c of a row, K sums of what term(c, sums) adds to
+// them: in 32 bits over runs of 64 columns and in 64 bits over the runs, so that
+// the rounding of a row of 2^30 columns (4 million a thread) is that of a short
+// one.  4096 rows of 32768: forward fp32 1132 us for 1091 with one sum in 32 bits,
+// backward bf16 820 (1442 without the loop's unrolling).
+constexpr int kNormRun = 64;
+
+template <int K, class Term>
+__device__ __forceinline__ void column_sums(int64_t C, float (&s)[K], Term term)
+{
+    double total[K] = {};
+    for (int64_t c = threadIdx.x; c < C;) {
+        float run[K] = {};
+        const int64_t end = min(C, c + kNormRun * kNormBlock);
+#pragma unroll 4
+        for (; c < end; c += kNormBlock) term(c, run);
+#pragma unroll
+        for (int k = 0; k < K; ++k) total[k] += run[k];
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = static_cast<float>(total[k]);
+}
 
 // One block per row, which it reads three times (the second and third come
 // from L1 or L2).
@@ -22,15 +48,14 @@ norm_fwd_rows(NormSource<Elem, kStreams> src, NormAffine aff, Elem* __restrict__
     group_sum_init<1>(group, buf[1]);
     for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
         const NormRow<Elem, kStreams> row(src, r);
-        float s[1] = {0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) s[0] += row.at(c);
+        float s[1];
+        column_sums(C, s, [&](int64_t c, float (&run)[1]) { run[0] += row.at(c); });
         group_sum(group, s, buf[0]);
         const float mean = s[0] / static_cast<float>(C);
-        s[0] = 0.0f;
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
+        column_sums(C, s, [&](int64_t c, float (&run)[1]) {
             const float d = row.at(c) - mean;
-            s[0] = fmaf(d, d, s[0]);
-        }
+            run[0] = fmaf(d, d, run[0]);
+        });
         group_sum(group, s, buf[1]);
         const float rstd = rsqrtf(s[0] / static_cast<float>(C) + eps);
         for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
@@ -61,16 +86,16 @@ norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kSt
         const NormRow<Elem, kStreams> row(src, r);
         const Elem* gr = g + r * g_stride;
         const float mean = mean_in[r], rstd = rstd_in[r];
-        float s[2] = {0.0f, 0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
+        float s[2];
+        column_sums(C, s, [&](int64_t c, float (&run)[2]) {
             const float gw = to_f32(gr[c]) * (aff.w ? load_any(aff.w, c, aff.dtype) : 1.0f);
-            s[0] += gw;
-            s[1] = fmaf(gw, (row.at(c) - mean) * rstd, s[1]);
-        }
+            run[0] += gw;
+            run[1] = fmaf(gw, (row.at(c) - mean) * rstd, run[1]);
+        });
         group_sum(group, s, buf);
         const float m1 = s[0] / static_cast<float>(C), m2 = s[1] / static_cast<float>(C);
-        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int64_t c = threadIdx.x; c < C; c += kNormBlock) {
+        float a[4];
+        column_sums(C, a, [&](int64_t c, float (&run)[4]) {
             const float gw = to_f32(gr[c]) * (aff.w ? load_any(aff.w, c, aff.dtype) : 1.0f);
             const float du = rstd * (gw - m1 - (row.at(c) - mean) * rstd * m2);
             if constexpr (kStreams == 1) {
@@ -78,11 +103,11 @@ norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kSt
             } else {
 #pragma unroll
                 for (int i = 0; i < kStreams; ++i) {
-                    a[i] = fmaf(du, to_f32(row.x[i * row.stream_stride + c]), a[i]);
+                    run[i] = fmaf(du, to_f32(row.x[i * row.stream_stride + c]), run[i]);
                     dx[(r * kStreams + i) * C + c] = from_f32<Elem>(row.h[i] * du);
                 }
             }
-        }
+        });
         if constexpr (kStreams > 1) {
             group_sum(group, a, buf_h);
             if (threadIdx.x == 0) {

@@ -157,3 +157,51 @@ def test_norm_gradients_of_tiny_and_huge_spreads():
             X, h = normal(g, 5, 4, C) * size, torch.rand(5, 4, device="cuda", generator=g)
             got = f.stream_norm_n4_backward(G, X, h, mean, rstd, w, b)
             ref.check(got, near_stream_norm(G, X, h, mean, rstd, w, b), (C, size, "streams"))
+
+
+# ---- rows wider than the rings hold --------------------------------------------------------
+
+# Terms that the wide rows' kernels add up in 32 bits at a time (64), the tree
+# over a block, and the roundings of a term.
+WIDE_DEPTH = 96
+
+
+@pytest.mark.parametrize("C", [(1 << 20) + 5, 1 << 22])
+@pytest.mark.parametrize("value", [0.1, 1.7])
+def test_sums_of_very_wide_rows(C, value):
+    """Rows of one value, whose running sum is rounded the same way again and
+    again: C / 256 additions in a row are off by hundreds of units in the last
+    place, and the bound here does not grow with C."""
+    g = gen(73)
+    x = torch.full((2, C), value, device="cuda")
+    x[1, ::2] = 0.5 * value
+    w, b = torch.full((C,), 1.5, device="cuda"), torch.full((C,), 0.25, device="cuda")
+    out = f.layer_norm(x, w, b, EPS)
+    ref.check(out, {k: (v, m, WIDE_DEPTH) for k, (v, m, _) in ref.layer_norm(x, w, b, EPS).items()}, C)
+    G = torch.full((2, C), 0.3, device="cuda")
+    got = f.layer_norm_backward(G, x, out["mean"], out["rstd"], w, b)
+    ref.check(got, near_layer_norm(G, x, out["mean"], out["rstd"], w, b, WIDE_DEPTH), C)
+    del got, G
+    X, h = x[:, None].expand(2, 4, C), torch.rand(2, 4, device="cuda", generator=g)
+    out = f.stream_norm_n4(X, h, w, b, EPS)
+    ref.check(out, {k: (v, m, WIDE_DEPTH) for k, (v, m, _) in ref.stream_norm(X, h, w, b, EPS).items()}, C)
+    G = torch.full((2, C), 0.3, device="cuda")
+    G[:, ::3] = 0.7
+    got = f.stream_norm_n4_backward(G, X, h, out["mean"], out["rstd"], w, b)
+    ref.check(got, near_stream_norm(G, X, h, out["mean"], out["rstd"], w, b, WIDE_DEPTH), C)
+
+
+@pytest.mark.parametrize("C", [10232, 10236, 10237, 10240, 10243, 10244, 10248, 12288, 12292, 12797, 14000])
+def test_stream_norm_where_fp32_rows_leave_the_rings(C):
+    """A stage of the backward holds the four streams and G, of the forward the
+    four streams: in fp32 they outgrow a block's shared memory below the
+    widest row of the 16-bit types."""
+    g = gen(C)
+    X, h = streams(300, C, g, torch.float32), torch.sigmoid(normal(g, 300, 4))
+    w, b = affine_of("float32", C, g, torch.float32)
+    for N in (5, 300):
+        out = f.stream_norm_n4(X[:N], h[:N], w, b, EPS)
+        ref.check(out, ref.stream_norm(X[:N], h[:N], w, b, EPS), (N, C))
+        G = normal(g, N, C)
+        got = f.stream_norm_n4_backward(G, X[:N], h[:N], out["mean"], out["rstd"], w, b)
+        ref.check(got, near_stream_norm(G, X[:N], h[:N], out["mean"], out["rstd"], w, b), (N, C))
