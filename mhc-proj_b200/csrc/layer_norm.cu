@@ -23,14 +23,9 @@
 namespace mhcp {
 
 constexpr int64_t kMaxRowGrid = int64_t{1} << 20;
-constexpr int64_t kParamChunks = 64;
-
-// Rows of partial sums at most: the row kernels' chunks, or the ring kernel's blocks.
-constexpr int64_t kMaxPartials = 1024;
-
 static int64_t norm_workspace(int64_t N, int64_t C)
 {
-    return std::min(std::max<int64_t>(N, 16), kMaxPartials) * 2 * C * static_cast<int64_t>(sizeof(float));
+    return norm_partial_rows(N, C) * 2 * C * static_cast<int64_t>(sizeof(float));
 }
 
 // Whether rows move in 16-byte pieces: whole pieces, aligned, and the
@@ -225,7 +220,7 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
         norm_bwd_rows<Elem, kStreams><<<static_cast<unsigned>(std::min(N, kMaxRowGrid)), kNormBlock, 0, stream>>>(
             gp, g_stride, src, mean, rstd, aff, dxp, dh, N, C);
         if (dw || db) {
-            rows = std::min(ceil_div(N, kParamRows), kParamChunks);
+            rows = param_chunks(N);
             const unsigned cols = static_cast<unsigned>(std::min<int64_t>(ceil_div(C, 32), int64_t{1} << 20));
             norm_param_partials<Elem, kStreams><<<dim3(cols, static_cast<unsigned>(rows)), 32 * kParamRows, 0, stream>>>(
                 gp, g_stride, src, mean, rstd, partials, N, C, ceil_div(N, rows));

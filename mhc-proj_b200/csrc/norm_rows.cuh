@@ -7,6 +7,7 @@
 #pragma once
 
 #include "norm_source.cuh"
+#include "ring_plan.h"
 
 namespace mhcp {
 
@@ -120,8 +121,7 @@ norm_bwd_rows(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kSt
 }
 
 // Partial sums of dw and db over one chunk of rows: partials[chunk][0 or 1][C].
-constexpr int kParamRows = 8;  // rows a block works on at once, 32 columns wide
-
+// A block works on kParamRows rows at once, 32 columns wide.
 template <class Elem, int kStreams>
 __global__ void __launch_bounds__(32 * kParamRows)
 norm_param_partials(const Elem* __restrict__ g, int64_t g_stride, NormSource<Elem, kStreams> src,

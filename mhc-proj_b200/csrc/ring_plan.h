@@ -143,4 +143,19 @@ inline RingPlan ring_plan(int64_t C, int elem, RowForm form)
     return p;
 }
 
+// Rows of partial sums of the parameters' gradients: one for every block of a
+// ring kernel (three for each of 160 SMs, whole periods of skewed rows), or of
+// the wide rows' kernels one for every chunk of rows.
+constexpr int64_t kMaxPartials = 3 * 160;
+constexpr int kParamRows = 8;
+constexpr int64_t kParamChunks = 64;
+
+inline int64_t param_chunks(int64_t N) { return std::min((N + kParamRows - 1) / kParamRows, kParamChunks); }
+
+// At most, for N rows of C elements of any type in any form.
+inline int64_t norm_partial_rows(int64_t N, int64_t C)
+{
+    return C > BwdShape<1, 2>::kWidest ? std::max<int64_t>(1, param_chunks(N)) : std::min(std::max<int64_t>(N, 16), kMaxPartials);
+}
+
 }  // namespace mhcp

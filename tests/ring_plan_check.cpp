@@ -52,6 +52,14 @@ int64_t check(int elem, RowForm form)
             CHECK(grid >= 1 && grid <= std::max<int64_t>(8, static_cast<int64_t>(p.blocks_per_sm) * 148));
             CHECK(form != kSkewed || grid * p.groups % (16 / elem) == 0);
         }
+        // the backward's blocks each have a row of the workspace
+        for (int64_t N : {1, 3, 17, 300, 500, 1 << 20}) {
+            const int64_t blocks = std::min(p.grid(N, elem, 148), kMaxPartials);
+            CHECK(blocks == p.grid(N, elem, 148) && blocks <= norm_partial_rows(N, C));
+            CHECK(param_chunks(N) <= norm_partial_rows(N, C));
+            const int64_t most = std::min(p.grid(N, elem, 1000), kMaxPartials);
+            CHECK(most <= norm_partial_rows(N, C) && (form != kSkewed || most * p.groups % (16 / elem) == 0));
+        }
     }
     return end;
 }

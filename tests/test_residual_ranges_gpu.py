@@ -205,3 +205,21 @@ def test_stream_norm_where_fp32_rows_leave_the_rings(C):
         G = normal(g, N, C)
         got = f.stream_norm_n4_backward(G, X[:N], h[:N], out["mean"], out["rstd"], w, b)
         ref.check(got, near_stream_norm(G, X[:N], h[:N], out["mean"], out["rstd"], w, b), (N, C))
+
+
+# ---- the backward's workspace ---------------------------------------------------------------
+
+def test_a_wide_backward_allocates_what_it_uses():
+    """256 rows of 2^20 elements: 32 rows of partial sums (0.25 GB) beside d_x
+    (0.5 GB), not one for every row (2 GB)."""
+    N, C = 256, 1 << 20
+    x = torch.ones(N, C, device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(C, device="cuda")
+    mean, rstd = torch.zeros(N, device="cuda"), torch.ones(N, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = f.layer_norm_backward(x, x, mean, rstd, w, w)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < x.numel() * 2 + 33 * 2 * C * 4 + 2 * C * 4 + (1 << 22)
+    assert bool((got["d_weight"] == N).all()) and bool((got["d_bias"] == N).all())
