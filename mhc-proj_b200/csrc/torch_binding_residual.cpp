@@ -231,12 +231,35 @@ py::dict layer_norm_backward(torch::Tensor G, torch::Tensor x, torch::Tensor mea
 
 // Dropout's key: a number (host), or a one-element int64 tensor that the kernel
 // reads when it is on the GPU.
+[[noreturn]] void bad_seed() { throw std::runtime_error("seed must be a whole number or a one-element int64 tensor"); }
+
+// The 64 bits of a whole number, signed or not (torch.initial_seed() is unsigned).
+int64_t seed_bits(const py::object& seed)
+{
+    const py::object number = py::reinterpret_steal<py::object>(PyNumber_Index(seed.ptr()));
+    if (!number) {
+        PyErr_Clear();
+        bad_seed();
+    }
+    int over = 0;
+    const long long bits = PyLong_AsLongLongAndOverflow(number.ptr(), &over);
+    if (!over) return bits;
+    const unsigned long long wide = over > 0 ? PyLong_AsUnsignedLongLong(number.ptr()) : 0;
+    if (over < 0 || PyErr_Occurred()) {
+        PyErr_Clear();
+        throw std::invalid_argument("seed must be between -2^63 and 2^64 - 1");
+    }
+    return static_cast<int64_t>(wide);
+}
+
 void check_seed(const py::object& seed)
 {
-    if (py::isinstance<py::int_>(seed)) return;
-    if (!THPVariable_Check(seed.ptr()) || py::cast<torch::Tensor>(seed).scalar_type() != torch::kInt64 ||
-        py::cast<torch::Tensor>(seed).numel() != 1)
-        throw std::runtime_error("seed must be a whole number or a one-element int64 tensor");
+    if (!THPVariable_Check(seed.ptr())) {
+        seed_bits(seed);
+    } else {
+        const torch::Tensor t = py::cast<torch::Tensor>(seed);
+        if (t.scalar_type() != torch::kInt64 || t.numel() != 1) bad_seed();
+    }
 }
 
 struct Seed {
@@ -245,8 +268,8 @@ struct Seed {
 
     Seed(const py::object& seed, const torch::TensorOptions& opts)
     {
-        if (py::isinstance<py::int_>(seed)) {
-            value = py::cast<int64_t>(seed);
+        if (!THPVariable_Check(seed.ptr())) {
+            value = seed_bits(seed);
             return;
         }
         held = py::cast<torch::Tensor>(seed);

@@ -8,6 +8,7 @@ import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
 
+import numpy
 import pytest
 import torch
 
@@ -223,3 +224,15 @@ def test_a_wide_backward_allocates_what_it_uses():
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < x.numel() * 2 + 33 * 2 * C * 4 + 2 * C * 4 + (1 << 22)
     assert bool((got["d_weight"] == N).all()) and bool((got["d_bias"] == N).all())
+
+
+# ---- seeds -------------------------------------------------------------------------------------
+
+def test_seeds_of_64_bits():
+    """What torch.initial_seed() may return: the key is the seed's 64 bits."""
+    x = torch.ones(1000, device="cuda")
+    for seed in (2 ** 63, 2 ** 64 - 5):
+        assert torch.equal(f.dropout(x, 0.5, seed, 1)["y"], f.dropout(x, 0.5, seed - 2 ** 64, 1)["y"])
+    assert torch.equal(f.dropout(x, 0.5, numpy.int64(-7), 1)["y"], f.dropout(x, 0.5, -7, 1)["y"])
+    m = mhc_proj.MHCDropout(0.5)
+    assert torch.equal(m(x, seed=2 ** 63 + 9), f.dropout(x, 0.5, 9 - 2 ** 63)["y"])
