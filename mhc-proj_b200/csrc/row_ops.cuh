@@ -11,8 +11,6 @@ namespace mhcp {
 
 inline bool known_dtype(int dtype) { return dtype >= MHC_DTYPE_F32 && dtype <= MHC_DTYPE_F16; }
 
-inline int elem_bytes(int dtype) { return dtype == MHC_DTYPE_F32 ? 4 : 2; }
-
 // Element i of an array whose type is known at run time only: the small
 // operands (per-token coefficients, a norm's weight and bias).
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype)
