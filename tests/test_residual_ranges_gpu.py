@@ -14,6 +14,7 @@ import torch
 
 import mhc_proj
 import residual_reference as ref
+from mhc_proj import residual
 from test_residual_gpu import DTYPES, EPS, affine_of, gen, leaf, mixing, normal, offset_copy, rows, same_bits, streams
 
 pytestmark = pytest.mark.gpu
@@ -206,6 +207,195 @@ def test_stream_norm_where_fp32_rows_leave_the_rings(C):
         G = normal(g, N, C)
         got = f.stream_norm_n4_backward(G, X[:N], h[:N], out["mean"], out["rstd"], w, b)
         ref.check(got, near_stream_norm(G, X[:N], h[:N], out["mean"], out["rstd"], w, b), (N, C))
+
+
+# ---- strides and offsets of batches that take the rings ---------------------------------------
+
+LAYOUTS = [(0, 8), (8, 0), (1, 0), (3, 5), (0, 1), (4, 4)]
+
+
+@pytest.mark.parametrize("offset,pad", LAYOUTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layer_norm_strides_of_many_rows(dtype, offset, pad):
+    """G lies as x does, and one element further on."""
+    g = gen(80)
+    for N, C in ((300, 256), (1500, 33), (1500, 1001), (1500, 1024), (300, 4096), (300, 4099), (300, 9000)):
+        x, G = rows(N, C, g, dtype), normal(g, N, C).to(dtype)
+        w, b = affine_of("same", C, g, dtype)
+        what = (dtype, offset, pad, N, C)
+        xs = offset_copy(x, offset, pad)
+        out = f.layer_norm(xs, w, b, EPS)
+        ref.check(out, ref.layer_norm(x, w, b, EPS), what)
+        want = near_layer_norm(G, x, out["mean"], out["rstd"], w, b)
+        for Gs in (offset_copy(G, offset, pad), offset_copy(G, offset + 1, pad), G):
+            ref.check(f.layer_norm_backward(Gs, xs, out["mean"], out["rstd"], w, b), want, what)
+
+
+@pytest.mark.parametrize("offset,pad", LAYOUTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_stream_norm_strides_of_many_rows(dtype, offset, pad):
+    g = gen(81)
+    for N, C in ((300, 256), (1500, 85), (700, 1001), (1500, 1024), (300, 4096), (300, 4099)):
+        X, G, h = streams(N, C, g, dtype), normal(g, N, C).to(dtype), torch.sigmoid(normal(g, N, 4))
+        w, b = affine_of("float32", C, g, dtype)
+        what = (dtype, offset, pad, N, C)
+        Xs, Gs = offset_copy(X, offset, pad), offset_copy(G, offset, pad)
+        Xt = offset_copy(X.transpose(0, 1), offset, pad).transpose(0, 1)  # stream-major
+        forward = ref.stream_norm(X, h, w, b, EPS)
+        out = f.stream_norm_n4(Xs, h, w, b, EPS)
+        backward = near_stream_norm(G, X, h, out["mean"], out["rstd"], w, b)
+        ref.check(out, forward, what)
+        ref.check(f.stream_norm_n4(Xt, h, w, b, EPS), forward, (what, "stream-major"))
+        for A, B in ((Xs, Gs), (Xt, G)):
+            ref.check(f.stream_norm_n4_backward(B, A, h, out["mean"], out["rstd"], w, b), backward, what)
+
+
+@pytest.mark.parametrize("offset,pad", LAYOUTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_stream_mix_strides_of_many_rows(dtype, offset, pad):
+    g = gen(82)
+    for N, C in ((1500, 25), (700, 49), (1500, 256), (700, 1001), (1500, 1024), (700, 4096), (700, 4099)):
+        X, y, G = streams(N, C, g, dtype), normal(g, N, C).to(dtype), normal(g, N, 4, C).to(dtype)
+        T, h = mixing(N, g), 2 * torch.sigmoid(normal(g, N, 4))
+        what = (dtype, offset, pad, N, C)
+        Xs, ys, Gs = offset_copy(X, offset, pad), offset_copy(y, offset, pad), offset_copy(G, offset, pad)
+        Xt, Gt = (offset_copy(t.transpose(0, 1), offset, pad).transpose(0, 1) for t in (X, G))
+        factor = ref.keep_factor(y.shape, 0.2, 4, 5, "cuda")
+        forward, backward = ref.stream_mix(X, T, y, h, factor), ref.stream_mix_backward(G, X, T, y, h, factor)
+        for A, B, z in ((Xs, Gs, ys), (Xt, Gt, y), (X, Gt, ys)):
+            ref.check(f.stream_mix_n4(A, T, z, h, 0.2, 4, 5), forward, what)
+            ref.check(f.stream_mix_n4_backward(B, A, T, z, h, 0.2, 4, 5), backward, what)
+
+
+@pytest.mark.parametrize("step", [1, 5, 8, 32])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_overlap(dtype, step):
+    """Windows of one array, `step` elements apart: rows that share elements."""
+    g = gen(83)
+    for N, C in ((700, 55), (700, 264)):
+        line, y, G = normal(g, (4 * N - 1) * step + C).to(dtype), normal(g, N, C).to(dtype), normal(g, N, C).to(dtype)
+        x, X = line.as_strided((N, C), (step, 1)), line.as_strided((N, 4, C), (4 * step, step, 1))
+        out = f.layer_norm(x, None, None, EPS)
+        ref.check(out, ref.layer_norm(x, None, None, EPS), (dtype, step, C))
+        ref.check(f.layer_norm_backward(G, x, out["mean"], out["rstd"]),
+                  near_layer_norm(G, x, out["mean"], out["rstd"], None, None), (dtype, step, C))
+        h, T = torch.sigmoid(normal(g, N, 4)), mixing(N, g)
+        out = f.stream_norm_n4(X, h, None, None, EPS)
+        ref.check(out, ref.stream_norm(X, h, None, None, EPS), (dtype, step, C))
+        ref.check(f.stream_norm_n4_backward(G, X, h, out["mean"], out["rstd"]),
+                  near_stream_norm(G, X, h, out["mean"], out["rstd"], None, None), (dtype, step, C))
+        factor = ref.keep_factor(y.shape, 0.2, 4, 5, "cuda")
+        ref.check(f.stream_mix_n4(X, T, x, h, 0.2, 4, 5), ref.stream_mix(X, T, x, h, factor), (dtype, step, C))
+        ref.check(f.stream_mix_n4_backward(X, X, T, x, h, 0.2, 4, 5), ref.stream_mix_backward(X, X, T, x, h, factor),
+                  (dtype, step, C))
+
+
+@pytest.mark.parametrize("C", [33, 96, 1001, 1024])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_operands_that_are_broadcast(dtype, C):
+    """One row for all tokens, one stream for a token's four: strides of zero."""
+    g = gen(C + 84)
+    N = 700
+    x, G = rows(1, C, g, dtype).expand(N, C), normal(g, 1, C).to(dtype).expand(N, C)
+    w, b = affine_of("same", C, g, dtype)
+    out = f.layer_norm(x, w, b, EPS)
+    ref.check(out, ref.layer_norm(x, w, b, EPS), (dtype, C))
+    ref.check(f.layer_norm_backward(G, x, out["mean"], out["rstd"], w, b),
+              near_layer_norm(G, x, out["mean"], out["rstd"], w, b), (dtype, C))
+    h, T = torch.sigmoid(normal(g, 1, 4)).expand(N, 4), mixing(1, g).expand(N, 4, 4)
+    factor = ref.keep_factor((N, C), 0.3, 8, 9, "cuda")
+    for X in (streams(1, C, g, dtype).expand(N, 4, C), rows(N, C, g, dtype)[:, None].expand(N, 4, C)):
+        out = f.stream_norm_n4(X, h, w, b, EPS)
+        ref.check(out, ref.stream_norm(X, h, w, b, EPS), (dtype, C))
+        ref.check(f.stream_norm_n4_backward(G, X, h, out["mean"], out["rstd"], w, b),
+                  near_stream_norm(G, X, h, out["mean"], out["rstd"], w, b), (dtype, C))
+        ref.check(f.stream_mix_n4(X, T, x, h, 0.3, 8, 9), ref.stream_mix(X, T, x, h, factor), (dtype, C))
+        G4 = G[:, None].expand(N, 4, C)
+        ref.check(f.stream_mix_n4_backward(G4, X, T, x, h, 0.3, 8, 9), ref.stream_mix_backward(G4, X, T, x, h, factor),
+                  (dtype, C))
+
+
+@pytest.mark.parametrize("cd", DTYPES)
+def test_coefficients_at_any_alignment(cd):
+    """T and h that start one element into a buffer, and columns of a wider array."""
+    g = gen(85)
+    for N, C in ((5, 96), (700, 96), (700, 1001)):
+        X, y, G = streams(N, C, g, torch.bfloat16), normal(g, N, C).bfloat16(), normal(g, N, 4, C).bfloat16()
+        T, h = mixing(N, g, cd), torch.sigmoid(normal(g, N, 4)).to(cd)
+        T1, h1 = offset_copy(T.reshape(1, -1), 1, 0).view(N, 4, 4), offset_copy(h.reshape(1, -1), 1, 0).view(N, 4)
+        for A, c in ((T1, h1), (T, h1), (T1, h), (offset_copy(T, 0, 3), offset_copy(h, 1, 20))):
+            assert same_bits(f.stream_mix_n4(X, A, y, c, 0.1, 5)["X"], f.stream_mix_n4(X, T, y, h, 0.1, 5)["X"])
+            got, want = (f.stream_mix_n4_backward(G, X, *t, 0.1, 5) for t in ((A, y, c), (T, y, h)))
+            assert all(same_bits(got[k], want[k]) for k in want)
+            out = f.stream_norm_n4(X, c)
+            assert same_bits(out["y"], f.stream_norm_n4(X, h)["y"])
+            got, want = (f.stream_norm_n4_backward(y, X, t, out["mean"], out["rstd"]) for t in (c, h))
+            assert all(same_bits(got[k], want[k]) for k in want)
+
+
+# ---- tensors of different types -------------------------------------------------------------
+
+@pytest.mark.parametrize("xt,yt", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                   (torch.float32, torch.float16), (torch.float16, torch.bfloat16)])
+def test_mix_of_streams_and_outputs_of_different_types(xt, yt):
+    """Streams kept in 32 bits around a 16-bit sublayer, and the other way round."""
+    g = gen(90)
+    for N, C in ((5, 96), (700, 1001)):
+        X, y = streams(N, C, g, xt), normal(g, N, C).to(yt)
+        T, h = mixing(N, g), 2 * torch.sigmoid(normal(g, N, 4))
+        factor = ref.keep_factor(y.shape, 0.1, 6, 7, "cuda")
+        out = f.stream_mix_n4(X, T, y, h, 0.1, 6, 7)
+        assert out["X"].dtype == xt
+        ref.check(out, ref.stream_mix(X, T, y, h, factor), (xt, yt, N, C))
+        for G in (normal(g, N, 4, C).to(xt), normal(g, N, 4, C).to(yt)):
+            got = f.stream_mix_n4_backward(G, X, T, y, h, 0.1, 6, 7)
+            assert got["d_X"].dtype == xt and got["d_y"].dtype == yt
+            ref.check(got, ref.stream_mix_backward(G, X, T, y, h, factor), (xt, yt, N, C))
+
+
+def test_a_layer_with_streams_in_32_bits_and_a_16_bit_sublayer():
+    g = gen(91)
+    X, h, W = leaf(normal(g, 6, 4, 96)), leaf(torch.sigmoid(normal(g, 6, 4))), leaf(normal(g, 96, 96).bfloat16() / 8)
+    T, norm, mix = mixing(6, g), mhc_proj.MHCStreamNormN4(96, device="cuda"), mhc_proj.MHCStreamMixN4()
+    out = mix(X, T, norm(X, h).bfloat16() @ W, h)
+    out.backward(torch.ones_like(out))
+    assert out.dtype == X.grad.dtype == h.grad.dtype == torch.float32 and W.grad.dtype == torch.bfloat16
+    n = f.stream_norm_n4(X.detach(), h.detach(), norm.weight.detach(), norm.bias.detach())["y"].bfloat16()
+    y = n @ W.detach()
+    assert same_bits(out.detach(), f.stream_mix_n4(X.detach(), T, y, h.detach())["X"])
+
+
+# ---- gradients of some of the inputs -----------------------------------------------------------
+
+def test_gradients_of_some_of_the_inputs():
+    """Frozen inputs get none, and the others the same bits."""
+    g = gen(92)
+    N, C = 37, 264
+    mix, norm, read = mhc_proj.MHCStreamMixN4(p=0.2), residual.MHCLayerNormFunction.apply, residual.MHCStreamNormN4Function.apply
+    x, X, G, G4 = normal(g, N, C), normal(g, N, 4, C), normal(g, N, C), normal(g, N, 4, C)
+    w, b, h, T = 1 + normal(g, C), normal(g, C), torch.rand(N, 4, device="cuda", generator=g), mixing(N, g)
+    for call, inputs, grad in ((norm, (x, w, b), G), (read, (X, h, w, b), G),
+                               (lambda *t: mix(*t, seed=3), (X, T, x, h), G4)):
+        leaves = [leaf(t) for t in inputs]
+        call(*leaves).backward(grad)
+        for some in range(1, 1 << len(inputs)):
+            part = [leaf(t) if some >> i & 1 else t for i, t in enumerate(inputs)]
+            call(*part).backward(grad)
+            for i, (p, full) in enumerate(zip(part, leaves)):
+                assert same_bits(p.grad, full.grad) if some >> i & 1 else p.grad is None
+
+
+def test_modules_on_empty_batches():
+    x, X, C = torch.empty(2, 0, 8, device="cuda"), torch.empty(0, 3, 4, 8, device="cuda"), 8
+    norm, read = mhc_proj.MHCLayerNorm(C, device="cuda"), mhc_proj.MHCStreamNormN4(C, device="cuda")
+    mix, x, X = mhc_proj.MHCStreamMixN4(p=0.5), leaf(x), leaf(X)
+    norm(x).sum().backward()
+    h, T, y = leaf(torch.empty(0, 3, 4, device="cuda")), torch.empty(0, 3, 4, 4, device="cuda"), leaf(X.detach()[:, :, 0])
+    (read(X, h).sum() + mix(X, T, y, h).sum() + mhc_proj.MHCDropout(0.5)(y).sum()).backward()
+    for t in (x, X, h, y):
+        assert t.grad.shape == t.shape
+    for m in (norm, read):
+        assert not bool(m.weight.grad.any()) and not bool(m.bias.grad.any())
 
 
 # ---- the backward's workspace ---------------------------------------------------------------
