@@ -322,11 +322,13 @@ MHC_API int mhc_sinkhorn_knopp_n4_hres_backward(const float* d_G, const float* d
  * Rows of C elements of one storage type (`dtype`), fp32 arithmetic and sums,
  * one rounding per output.  A row's elements are contiguous; strides are in
  * elements and non-negative; outputs are contiguous.  1 <= C <= 2^30 is any
- * width, 0 <= N < 2^31, and any alignment is accepted (rows whose starts are
- * 16-byte aligned and whose width is a multiple of 16 bytes move in 16-byte
- * pieces).  Tensors must lie in memory as a whole: the bytes between the rows of
- * a strided one may be read (their values are not used).  No reference
- * counterparts. */
+ * width, 0 <= N < 2^31.  Any alignment to the element is accepted (rows whose
+ * starts are 16-byte aligned and whose width is a multiple of 16 bytes move in
+ * 16-byte pieces); an array that starts between two elements, a workspace or
+ * statistics off 4 bytes or a d_seed off 8 is refused.  Outputs overlap neither
+ * one another nor an input (but for mhc_dropout's).  Tensors must lie in memory
+ * as a whole: the bytes between the rows of a strided one may be read (their
+ * values are not used).  No reference counterparts. */
 
 /* y = (x - mean) * rstd * w + b per row, rstd = 1 / sqrt(var + eps) with the
  * biased variance.  Row k of x starts at element k * x_stride.  d_w and d_b

@@ -82,7 +82,8 @@ dropout_kernel(const Elem* x, Elem* y, int64_t count, Dropout d)
 template <class Elem, bool kVec, int kGroups>
 static int dropout_launch(const Elem* x, Elem* y, int64_t count, const Dropout& d, cudaStream_t stream)
 {
-    const int64_t blocks = ceil_div(count, 8 * kDropBlock * kGroups);
+    constexpr int64_t kPerBlock = 8 * kDropBlock * kGroups;
+    const int64_t blocks = count / kPerBlock + (count % kPerBlock != 0);
     if (blocks > 0x7fffffff) return MHC_ERR_INVALID_VALUE;
     dropout_kernel<Elem, kVec, kGroups><<<static_cast<unsigned>(blocks), kDropBlock, 0, stream>>>(x, y, count, d);
     return static_cast<int>(cudaGetLastError());
@@ -108,7 +109,8 @@ using namespace mhcp;
 extern "C" int mhc_dropout(const void* d_x, void* d_y, int dtype, int64_t count, double p, int64_t seed,
                            const int64_t* d_seed, int64_t offset, cudaStream_t stream)
 {
-    if (count < 0 || !(p >= 0.0 && p <= 1.0) || !known_dtype(dtype) || (count > 0 && (!d_x || !d_y)))
+    if (count < 0 || !(p >= 0.0 && p <= 1.0) || !known_dtype(dtype) || (count > 0 && (!d_x || !d_y)) ||
+        !at_elements(dtype, d_x, d_y) || !at_element(d_seed, 8))
         return MHC_ERR_INVALID_VALUE;
     if (count == 0) return MHC_OK;
     const Dropout d = make_dropout(p, seed, d_seed, offset);

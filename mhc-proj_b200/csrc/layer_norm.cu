@@ -132,7 +132,9 @@ static int norm_forward(const void* x, int64_t stride, int64_t stream_stride, in
                         int64_t N, int64_t C, cudaStream_t stream)
 {
     if (!rows_ok(N, C) || stride < 0 || stream_stride < 0 || !known_dtype(dtype) || !known_dtype(h_dtype) ||
-        !known_dtype(w_dtype) || !(eps >= 0.0f) || (N > 0 && (!x || !y || (kStreams > 1 && !h))))
+        !known_dtype(w_dtype) || !(eps >= 0.0f) || (N > 0 && (!x || !y || (kStreams > 1 && !h))) ||
+        !at_elements(dtype, x, y) || !at_elements(h_dtype, h) || !at_elements(w_dtype, w, b) ||
+        !at_elements(MHC_DTYPE_F32, mean, rstd))
         return MHC_ERR_INVALID_VALUE;
     if (N == 0) return MHC_OK;
     const NormAffine aff{w, b, w_dtype};
@@ -241,7 +243,9 @@ static int norm_backward(const void* g, int64_t g_stride, const void* x, int64_t
 {
     if (!rows_ok(N, C) || g_stride < 0 || stride < 0 || stream_stride < 0 || !known_dtype(dtype) ||
         !known_dtype(h_dtype) || !known_dtype(w_dtype) ||
-        (N > 0 && (!g || !x || !mean || !rstd || !dx || (kStreams > 1 && (!h || !dh)))))
+        (N > 0 && (!g || !x || !mean || !rstd || !dx || (kStreams > 1 && (!h || !dh)))) ||
+        !at_elements(dtype, g, x, dx) || !at_elements(h_dtype, h, dh) || !at_elements(w_dtype, w, dw, db) ||
+        !at_elements(MHC_DTYPE_F32, mean, rstd, workspace))
         return MHC_ERR_INVALID_VALUE;
     if (N > 0 && (dw || db) && (!workspace || workspace_bytes < norm_workspace(N, C))) return MHC_ERR_INVALID_VALUE;
     if (N == 0 && !dw && !db) return MHC_OK;

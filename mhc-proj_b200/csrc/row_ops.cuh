@@ -11,6 +11,16 @@ namespace mhcp {
 
 inline bool known_dtype(int dtype) { return dtype >= MHC_DTYPE_F32 && dtype <= MHC_DTYPE_F16; }
 
+// Whether an array (which may be null) starts at one of its elements' addresses:
+// a load from another one is a fault.
+inline bool at_element(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+template <class... Pointers>
+inline bool at_elements(int dtype, Pointers... p)
+{
+    return (at_element(p, dtype == MHC_DTYPE_F32 ? 4 : 2) && ...);
+}
+
 // Element i of an array whose type is known at run time only: the small
 // operands (per-token coefficients, a norm's weight and bias).
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype)

@@ -322,11 +322,12 @@ static int mix_backward(const void* g, int64_t g_stride, int64_t g_stream_stride
 
 static bool mix_args_ok(const void* X, int64_t token_stride, int64_t stream_stride, const void* y, int64_t y_stride,
                         int dtype, const void* T, int T_dtype, const void* h, int h_dtype, double p, int64_t N,
-                        int64_t C)
+                        int64_t C, const int64_t* d_seed)
 {
     return rows_ok(N, C) && token_stride >= 0 && stream_stride >= 0 && y_stride >= 0 && known_dtype(dtype) &&
            known_dtype(T_dtype) && known_dtype(h_dtype) && p >= 0.0 && p <= 1.0 &&
-           (N == 0 || (X && y && T && h));
+           (N == 0 || (X && y && T && h)) && at_elements(dtype, X, y) && at_elements(T_dtype, T) &&
+           at_elements(h_dtype, h) && at_element(d_seed, 8);
 }
 
 // The coefficients in the form that is read 16 bytes at a time.
@@ -344,8 +345,8 @@ extern "C" int mhc_stream_mix_n4(const void* d_X, int64_t token_stride, int64_t 
                                  int h_dtype, void* d_out, double p, int64_t seed, const int64_t* d_seed,
                                  int64_t offset, int64_t N, int64_t C, cudaStream_t stream)
 {
-    if (!mix_args_ok(d_X, token_stride, stream_stride, d_y, y_stride, dtype, d_T, T_dtype, d_h, h_dtype, p, N, C) ||
-        (N > 0 && !d_out))
+    if (!mix_args_ok(d_X, token_stride, stream_stride, d_y, y_stride, dtype, d_T, T_dtype, d_h, h_dtype, p, N, C, d_seed) ||
+        (N > 0 && !d_out) || !at_elements(dtype, d_out))
         return MHC_ERR_INVALID_VALUE;
     if (N == 0) return MHC_OK;
     const Dropout d = make_dropout(p, seed, d_seed, offset);
@@ -371,8 +372,9 @@ extern "C" int mhc_stream_mix_n4_backward(const void* d_G, int64_t g_token_strid
                                           double p, int64_t seed, const int64_t* d_seed, int64_t offset, int64_t N,
                                           int64_t C, cudaStream_t stream)
 {
-    if (!mix_args_ok(d_X, token_stride, stream_stride, d_y, y_stride, dtype, d_T, T_dtype, d_h, h_dtype, p, N, C) ||
-        g_token_stride < 0 || g_stream_stride < 0 || (N > 0 && (!d_G || !d_dX || !d_dT || !d_dy || !d_dh)))
+    if (!mix_args_ok(d_X, token_stride, stream_stride, d_y, y_stride, dtype, d_T, T_dtype, d_h, h_dtype, p, N, C, d_seed) ||
+        g_token_stride < 0 || g_stream_stride < 0 || (N > 0 && (!d_G || !d_dX || !d_dT || !d_dy || !d_dh)) ||
+        !at_elements(dtype, d_G, d_dX, d_dy) || !at_elements(T_dtype, d_dT) || !at_elements(h_dtype, d_dh))
         return MHC_ERR_INVALID_VALUE;
     if (N == 0) return MHC_OK;
     const Dropout d = make_dropout(p, seed, d_seed, offset);
