@@ -262,8 +262,10 @@ mix_fwd_ring(MixIn<Elem> in, RowSpan x_span, RowSpan y_span, Elem* __restrict__ 
 }
 
 // The backward pass: a warp takes whole tokens (of kVec 32 / lanes at a time),
-// chunk after chunk.
-template <class Elem, bool kVec, bool kWide>
+// chunk after chunk.  kLong: tokens of more than a run of chunks (a kernel of its own:
+// the sums over runs cost registers, and with them the third block of an SM:
+// 20000 tokens of 512 bf16 73 us for 49).
+template <class Elem, bool kVec, bool kWide, bool kLong>
 __global__ void __launch_bounds__(kMixRingBlock)
 mix_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stride, RowSpan g_span, MixIn<Elem> in,
              RowSpan x_span, RowSpan y_span, Elem* __restrict__ dx, void* __restrict__ dT, Elem* __restrict__ dy,
@@ -311,6 +313,8 @@ mix_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stri
         const int64_t r = group * per_warp + mine;
         const MixCoef k = mix_coef<kWide>(in, min(r, N - 1));
         float2 acc[20];
+        float sums[20];
+        double total = 0.0;  // of the runs before
 #pragma unroll
         for (int i = 0; i < 20; ++i) acc[i] = both(0.0f);
         for (int s = 0; s < chunks; ++s) {
@@ -376,11 +380,21 @@ mix_bwd_ring(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_stri
             if constexpr (!kVec) __syncwarp();  // others have read what is copied over
             fill(stage);
             stage = (stage + 1) % kMixBwdStages;
+            if constexpr (kLong) {
+                constexpr int run = kMixRun / (Chunk::kPairs * Chunk::kSteps);  // chunks
+                if (s % run == run - 1 && s + 1 < chunks) {
+#pragma unroll
+                    for (int i = 0; i < 20; ++i) {
+                        sums[i] = acc[i].x + acc[i].y;
+                        acc[i] = both(0.0f);
+                    }
+                    total += warp_sum20(sums);
+                }
+            }
         }
-        float sums[20];
 #pragma unroll
         for (int i = 0; i < 20; ++i) sums[i] = acc[i].x + acc[i].y;
-        put_token_sums(in, r, r < N, lane, lanes, sums, dT, dh);
+        put_token_sums<kLong>(in, r, r < N, lane, lanes, sums, dT, dh, total);
     }
 }
 

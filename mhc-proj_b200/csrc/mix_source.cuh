@@ -89,18 +89,31 @@ __device__ __forceinline__ float warp_sum20(const float (&a)[20])
     return lane < 16 ? b[0] : rest[0];
 }
 
-// Writes the sums of a token that `lanes` lanes share, from each lane's part.
+// A thread adds up a token's terms for its 20 sums in 32 bits over runs of so many
+// columns' pairs; the runs are added up in 64 bits, so that the rounding of a
+// token of 2^30 columns is that of a short one.
+constexpr int kMixRun = 256;
+
+// Sum number `mine` (warp_sum20's order) of a token.
 template <class Elem>
+__device__ __forceinline__ void put_token_sum(const MixIn<Elem>& in, int64_t r, int mine, float sum, void* dT, void* dh)
+{
+    if (mine < 16)
+        store_any(dT, 16 * r + mine, in.T_dtype, sum);
+    else if (mine < 20)
+        store_any(dh, 4 * r + mine - 16, in.h_dtype, sum);
+}
+
+// Writes the sums of a token that `lanes` lanes share, from each lane's part
+// (kLong: of the last run, and lane l has sum l of the runs before it).
+template <bool kLong = false, class Elem>
 __device__ __forceinline__ void put_token_sums(const MixIn<Elem>& in, int64_t r, bool live, int lane, int lanes,
-                                               float (&v)[20], void* dT, void* dh)
+                                               float (&v)[20], void* dT, void* dh, double before = 0.0)
 {
     if (lanes == 32) {
-        const float sum = warp_sum20(v);
-        if (!live) return;
-        if (lane < 16)
-            store_any(dT, 16 * r + lane, in.T_dtype, sum);
-        else if (lane < 20)
-            store_any(dh, 4 * r + lane - 16, in.h_dtype, sum);
+        float sum = warp_sum20(v);
+        if constexpr (kLong) sum = static_cast<float>(before + sum);
+        if (live) put_token_sum(in, r, lane, sum, dT, dh);
         return;
     }
     for (int m = lanes >> 1; m > 0; m >>= 1) {

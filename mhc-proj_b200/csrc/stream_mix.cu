@@ -151,6 +151,8 @@ mix_bwd_direct(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_st
     const bool live = r < N;
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     float2 acc[20];
+    float sums[20];
+    double total = 0.0;
 #pragma unroll
     for (int i = 0; i < 20; ++i) acc[i] = both(0.0f);
     if (live) {
@@ -195,9 +197,16 @@ mix_bwd_direct(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_st
                 }
                 map.store(dx + (4 * r + j) * C, s, b);
             }
+            constexpr int run = kMixRun / kPairs;  // steps: only a token of a whole block has more
+            if (s % run != run - 1 || s + 1 == steps) continue;
+#pragma unroll
+            for (int i = 0; i < 20; ++i) {
+                sums[i] = acc[i].x + acc[i].y;
+                acc[i] = both(0.0f);
+            }
+            total += warp_sum20(sums);
         }
     }
-    float sums[20];
 #pragma unroll
     for (int i = 0; i < 20; ++i) sums[i] = acc[i].x + acc[i].y;
     if (warps <= 1) {
@@ -205,16 +214,13 @@ mix_bwd_direct(const Elem* __restrict__ g, int64_t g_stride, int64_t g_stream_st
         return;
     }
     // one token in the block: its warps' sums in warp order
-    const float sum = warp_sum20(sums);
-    if (lane < 20) part[threadIdx.x >> 5][lane] = sum;
+    total += warp_sum20(sums);
+    if (lane < 20) part[threadIdx.x >> 5][lane] = static_cast<float>(total);
     __syncthreads();
     if (threadIdx.x >= 20) return;
     float all = 0.0f;
     for (int w = 0; w < warps; ++w) all += part[w][lane];
-    if (lane < 16)
-        store_any(dT, 16 * r + lane, in.T_dtype, all);
-    else
-        store_any(dh, 4 * r + lane - 16, in.h_dtype, all);
+    put_token_sum(in, r, lane, all, dT, dh);
 }
 
 static bool aligned_streams(const void* p, int64_t stride, int64_t stream_stride, int elem)
@@ -239,7 +245,7 @@ static int mix_threads(int64_t want, int least, int most)
 
 // Rows of single elements narrower than this take the direct kernels, where a
 // token takes 8 to 32 lanes; the ring kernels give it a warp.  65536 tokens, bf16,
-// forward / backward us: 25 wide 21 / 66 direct, 28 / 105 in the ring; 99 wide
+// forward / backward us: 25 wide 21 / 49 direct, 28 / 105 in the ring; 99 wide
 // 76 / 251 direct, 55 / 111 in the ring.
 constexpr int64_t kMixNarrow = 48;
 
@@ -271,13 +277,13 @@ static int mix_forward(const MixIn<Elem>& in, void* out, const Dropout& d, int64
     return static_cast<int>(cudaGetLastError());
 }
 
-template <class Elem, bool kVec, bool kWide>
+template <class Elem, bool kVec, bool kWide, bool kLong>
 static int mix_backward_ring(const Elem* g, int64_t g_stride, int64_t g_stream_stride, const MixIn<Elem>& in, Elem* dx,
                              void* dT, Elem* dy, void* dh, const Dropout& d, int64_t N, int64_t C, cudaStream_t stream)
 {
     using Chunk = MixChunk<Elem, kVec>;
     constexpr int warps = kMixRingBlock / 32, smem = warps * kMixBwdStages * 9 * Chunk::kPlace;
-    const cudaError_t e = allow_smem<sizeof(MixMasks)>(mix_bwd_ring<Elem, kVec, kWide>, smem);
+    const cudaError_t e = allow_smem<sizeof(MixMasks)>(mix_bwd_ring<Elem, kVec, kWide, kLong>, smem);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int lanes = kVec ? mix_threads(C / Chunk::K, 1, 32) : 32;
     // Two blocks an SM (65536 tokens of 2048, bf16: 595 us, with three 675), or
@@ -285,7 +291,7 @@ static int mix_backward_ring(const Elem* g, int64_t g_stride, int64_t g_stream_s
     // or single elements take more instructions.
     const int blocks = kVec && Chunk::count(static_cast<int>(C), lanes) > 2 ? 2 : 3;
     const int64_t grid = std::min<int64_t>(ceil_div(ceil_div(N, 32 / lanes), warps), blocks * sm_count());
-    mix_bwd_ring<Elem, kVec, kWide><<<static_cast<unsigned>(grid), kMixRingBlock, smem, stream>>>(
+    mix_bwd_ring<Elem, kVec, kWide, kLong><<<static_cast<unsigned>(grid), kMixRingBlock, smem, stream>>>(
         g, g_stride, g_stream_stride, span_of(g, N, g_stride, 4, g_stream_stride, C), in,
         span_of(in.x, N, in.stride, 4, in.stream_stride, C), span_of(in.y, N, in.y_stride, 1, 0, C), dx, dT, dy, dh, d, N,
         static_cast<int>(C), lanes);
@@ -304,9 +310,16 @@ static int mix_backward(const void* g, int64_t g_stride, int64_t g_stream_stride
     // A warp per token once there are four tokens for every SM, else a block
     // (bf16, 4096 wide: 300 tokens 14.0 us a warp each, 11.3 a block each; 1000
     // tokens 23.6 and 30.4).
-    if (N >= 4 * sm_count() && !narrow)
-        return pieces ? mix_backward_ring<Elem, true, kWide>(gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, C, stream)
-                      : mix_backward_ring<Elem, false, kWide>(gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, C, stream);
+    if (N >= 4 * sm_count() && !narrow) {
+        auto ring = [&](auto vec, auto is_long) {
+            return mix_backward_ring<Elem, decltype(vec)::value, kWide, decltype(is_long)::value>(
+                gp, g_stride, g_stream_stride, in, dxp, dT, dyp, dh, d, N, C, stream);
+        };
+        using std::false_type, std::true_type;
+        // a run is 256 pairs of columns a lane
+        if (C > 2 * 32 * kMixRun) return pieces ? ring(true_type{}, true_type{}) : ring(false_type{}, true_type{});
+        return pieces ? ring(true_type{}, false_type{}) : ring(false_type{}, false_type{});
+    }
     const int t = narrow ? mix_threads(ceil_div(C, 4), 8, 32)
                          : mix_threads(pieces ? C * static_cast<int64_t>(sizeof(Elem)) / 16 : ceil_div(C, 4), 32, kMixBlock);
     const int tokens = t <= 32 ? 128 / t : 1;

@@ -193,6 +193,42 @@ def test_sums_of_very_wide_rows(C, value):
     ref.check(got, near_stream_norm(G, X, h, out["mean"], out["rstd"], w, b, WIDE_DEPTH), C)
 
 
+# Terms of a coefficient's gradient that a thread adds up in 32 bits at a time (64
+# steps of at most four), the tree over a warp or block, and the roundings of a term.
+MIX_DEPTH = 288
+
+
+@pytest.mark.parametrize("N,C,dtype", [(3, 1 << 22, torch.float32), (3, (1 << 22) + 3, torch.float32),
+                                       (600, 1 << 18, torch.bfloat16), (600, (1 << 18) + 1, torch.bfloat16),
+                                       (600, 1 << 18, torch.float32)])
+def test_coefficient_gradients_of_very_wide_tokens(N, C, dtype):
+    """Equal products, whose running sum is rounded the same way again and
+    again: a token's sums for T and h_post, by a block (few tokens) or a warp."""
+    g = gen(74)
+    X, y = (torch.full((1, *s, C), 0.9, device="cuda").to(dtype).expand(N, *s, C) for s in ((4,), ()))
+    G = torch.full((1, 4, C), 1.1, device="cuda").to(dtype).expand(N, 4, C)
+    T, h = mixing(N, g), torch.sigmoid(normal(g, N, 4))
+    got = f.stream_mix_n4_backward(G, X, T, y, h)
+    for part in (slice(0, 2), slice(N - 1, N)):
+        t = [v[part] for v in (G, X, T, y, h)]
+        want = ref.stream_mix_backward(*t, torch.ones(t[3].shape, dtype=torch.float64, device="cuda"))
+        ref.check({k: v[part] for k, v in got.items()},
+                  {k: (v, m, MIX_DEPTH if k in ("d_T", "d_h_post") else d) for k, (v, m, d) in want.items()}, (N, C))
+
+
+@pytest.mark.parametrize("C", [16384, 16385, 16392, 40000, 40001])
+def test_mix_where_tokens_take_several_runs(C):
+    g = gen(C)
+    N, dtype = 600, torch.bfloat16
+    X, y, G = streams(N, C, g, dtype), normal(g, N, C).to(dtype), normal(g, N, 4, C).to(dtype)
+    T, h = mixing(N, g), 2 * torch.sigmoid(normal(g, N, 4))
+    factor = ref.keep_factor(y.shape, 0.2, 4, 5, "cuda")
+    ref.check(f.stream_mix_n4(X, T, y, h, 0.2, 4, 5), ref.stream_mix(X, T, y, h, factor), C)
+    for n in (600, 5):
+        t = [v[:n] for v in (G, X, T, y, h)]
+        ref.check(f.stream_mix_n4_backward(*t, 0.2, 4, 5), ref.stream_mix_backward(*t, factor[:n]), (n, C))
+
+
 @pytest.mark.parametrize("C", [10232, 10236, 10237, 10240, 10243, 10244, 10248, 12288, 12292, 12797, 14000])
 def test_stream_norm_where_fp32_rows_leave_the_rings(C):
     """A stage of the backward holds the four streams and G, of the forward the
