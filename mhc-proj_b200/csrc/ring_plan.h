@@ -55,9 +55,10 @@ MHCP_BOTH inline int part_pitch(int C) { return (C + 15) / 8 * 8; }
 // The ring kernels' shapes by width: elements of a row per thread, the most
 // threads of a group (their product is the widest row), rows a turn, and
 // whether the parameters stay in registers.  512 threads of an SM have 128
-// registers each: the shapes of the widths up to 4096 fit in them but for a
-// pair (16 elements a thread for the four streams' gradients, which spill: 506 us
-// against 440, 65536 x 2048 bf16); wider rows spill what 32 elements a thread need.
+// registers each.  One stream's shapes of up to 8192 columns and four streams' of
+// up to 4096 fit in them (16 elements a thread for the four streams' gradients
+// spill, so narrower rows do not take them: 506 us against 440, 65536 x 2048 bf16);
+// wider rows spill what they need.
 template <int kStreams, int kWidth>
 struct FwdShape {
     static constexpr int kElems = kWidth ? 32 : 16, kTurn = kStreams == 1 && !kWidth ? 2 : 1;
