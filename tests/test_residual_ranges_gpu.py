@@ -47,7 +47,8 @@ print("ok")
 
 
 def first_call(case):
-    env = dict(os.environ, PYTHONPATH=os.pathsep.join([HERE, os.path.join(os.path.dirname(HERE), "mhc-proj_b200")]))
+    path = [HERE, os.path.join(os.path.dirname(HERE), "mhc-proj_b200"), os.environ.get("PYTHONPATH", "")]
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(filter(None, path)))
     run = subprocess.run([sys.executable, "-c", FIRST_CALL, *map(str, case)], env=env, cwd=HERE, capture_output=True,
                          text=True, timeout=300)
     return run.stdout.strip() if run.returncode == 0 else run.stderr[-600:]
